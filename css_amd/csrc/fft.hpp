@@ -11,8 +11,8 @@
 #pragma once
 #include "common.hpp"
 
-// complex numbers are 2-vectors so that the butterflies compile to packed FP32 (v_pk_add_f32 / v_pk_fma_f32 with
-// op_sel / neg modifiers): one instruction per complex add, two per complex multiply
+// complex numbers are 2-vectors; the build keeps packed FP32 instructions out (Makefile, NO_PK32), so a complex add is two
+// instructions and a complex multiply four
 typedef float cplx __attribute__((ext_vector_type(2)));
 DEV cplx cmul(cplx a, cplx b) {  // a.xx * b + a.yy * (-b.y, b.x)
   return __builtin_elementwise_fma(a.xx, b, a.yy * cplx{-b.y, b.x});

@@ -9,7 +9,7 @@ mode=$1; shift
 mkdir -p build/abl
 for m in "$@"; do
   if [ "$mode" = build ]; then
-    fl="-DA2_ABL=$m"; [ "$m" = stamps ] && fl="-DA2_STAMPS"; hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-function $fl -c css_amd/csrc/attn.hip -o build/abl/attn_$m.o
+    fl="-DA2_ABL=$m"; [ "$m" = stamps ] && fl="-DA2_STAMPS"; hipcc -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-function $fl -c css_amd/csrc/attn.hip -o build/abl/attn_$m.o
     objs=$(ls css_amd/csrc/*.o | grep -v '/attn.o')
     hipcc -shared -fPIC --offload-arch=gfx950 -o build/abl/lib_$m.so $objs build/abl/attn_$m.o
   else

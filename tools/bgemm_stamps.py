@@ -1,5 +1,5 @@
 """Per-workgroup phase timeline of one bgemm launch.  Needs a library whose bgemm.o was built with -DBG_STAMPS:
-  cd css_amd/csrc && hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -I../../include -DBG_STAMPS -c bgemm.hip -o /tmp/bgs.o
+  cd css_amd/csrc && hipcc -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC --offload-arch=gfx950 -I../../include -DBG_STAMPS -c bgemm.hip -o /tmp/bgs.o
   hipcc -shared -fPIC --offload-arch=gfx950 -o ../../build/lib_stamps.so $(ls *.o | grep -v '^bgemm.o$') /tmp/bgs.o
 python tools/bgemm_stamps.py build/lib_stamps.so M N K akm bkm af bf [splits]"""
 import ctypes as C, os, sys

@@ -1,5 +1,5 @@
 """Per-wave phase timeline of one csship_attn_dvdk launch.  Needs a library whose attnbwd.o was built with -DDV_STAMPS:
-  cd css_amd/csrc && hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -I../../include -DDV_STAMPS -c attnbwd.hip -o probe/attnbwd_st.o
+  cd css_amd/csrc && hipcc -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC --offload-arch=gfx950 -I../../include -DDV_STAMPS -c attnbwd.hip -o probe/attnbwd_st.o
   hipcc -shared -fPIC --offload-arch=gfx950 -o probe/libst.so $(ls *.o | grep -v '^attnbwd.o$') probe/attnbwd_st.o
 python tools/dvdk_stamps.py css_amd/csrc/probe/libst.so [B H T]"""
 import ctypes as C, os, sys

@@ -5,8 +5,8 @@
 set -u
 cd css_amd/csrc
 for abl in 0 1 2 4 8 16 32 3 35 39 63; do
-  hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-function -DMX_ABL=$abl -c ffnw.hip -o ffnw.o 2>/dev/null
+  hipcc -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-function -DMX_ABL=$abl -c ffnw.hip -o ffnw.o 2>/dev/null
   hipcc -shared -fPIC --offload-arch=gfx950 -o libcsship.so *.o
   echo "MX_ABL=$abl: $(cd ../.. && timeout -k 10 200 python tools/bench_large.py --blocks 1 2>/dev/null | grep -E '^ffn_mxfp8|^ffn_wide')" | tr '\n' ' '; echo
 done
-hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-function -c ffnw.hip -o ffnw.o && hipcc -shared -fPIC --offload-arch=gfx950 -o libcsship.so *.o
+hipcc -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-function -c ffnw.hip -o ffnw.o && hipcc -shared -fPIC --offload-arch=gfx950 -o libcsship.so *.o

@@ -1,5 +1,5 @@
 """Per-wave phase timeline of one csship_head_pit launch.  Needs a library whose headpit.o was built with -DHP_STAMPS:
-  cd css_amd/csrc && mkdir -p probe && hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -I../../include -DHP_STAMPS -c headpit.hip -o probe/headpit_st.o
+  cd css_amd/csrc && mkdir -p probe && hipcc -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC --offload-arch=gfx950 -I../../include -DHP_STAMPS -c headpit.hip -o probe/headpit_st.o
   hipcc -shared -fPIC --offload-arch=gfx950 -o probe/libhp.so $(ls *.o | grep -v '^headpit.o$') probe/headpit_st.o
 python tools/headpit_stamps.py css_amd/csrc/probe/libhp.so"""
 import ctypes as C, os, sys

@@ -7,7 +7,7 @@ operations in flight, so a kernel that prefetches N loads ahead ends up waiting 
 (round 5: the chain kernel's W2 passes ended on vmcnt(1) where vmcnt(8) was meant).  A kernel whose loop shows many small
 N next to its intended prefetch depth is a candidate.
 
-    hipcc -O3 -std=c++17 --offload-arch=gfx950 --cuda-device-only -S css_amd/csrc/panel.hip -o /tmp/panel.s
+    hipcc -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 --offload-arch=gfx950 --cuda-device-only -S css_amd/csrc/panel.hip -o /tmp/panel.s
     python tools/isa_waits.py /tmp/panel.s [name filter]
 """
 import collections
