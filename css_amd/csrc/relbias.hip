@@ -1,0 +1,818 @@
+// Attention with a learned bias per (bucket of the key-query distance, head): forward, and the backward that recomputes
+// the probabilities.  The formulas are in include/csship.h (csship_relbias).
+//
+// Matrix products are v_mfma_f32_32x32x16 (lane l of an operand: row l & 31, eight k values 8 (l >> 5) ..; accumulator register
+// r of lane l: row 8 (r >> 2) + 4 (l >> 5) + (r & 3), column l & 31).  Scores are computed TRANSPOSED where the queries are
+// what a wave owns, S^T[key, query] = K Q^T: a lane then holds one query and four consecutive keys per register group, so
+//   * row maxima and sums are register sums plus ONE exchange between the two half waves;
+//   * the rounded probabilities are already the B operand of the next product: its reduction index may run over the keys in
+//     any order as long as both operands agree, and register group order (keys 4 hi .. + 3, 8 + 4 hi .. + 3) is the order in
+//     which two ds_read_b64_tr_b16 deliver V^T;
+//   * the bias of the four keys is four consecutive floats of the head's table, spread over distances once per workgroup in
+//     LDS, and goes into the product as its initial accumulator: no addition per score.  Tiles wholly beyond the largest
+//     distance start from a constant.
+#include "common.hpp"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr float RB_LOG2E = 1.4426950408889634f, RB_LN2 = 0.6931471805599453f;
+constexpr int RB_PAD = 96;          // entries of the spread table beyond the largest distance on each side: a 64 x 32 tile that
+                                    // is not wholly beyond it reaches at most 64 + 32 - 2 further
+constexpr float RB_BIG = 1048576.f; // table entries at or below -2^20 ban their distances; entries above 2^20 count as 2^20
+constexpr int RB_MAX_POS = 1 << 28;  // lengths and offsets stay below it: distances in 32 bits
+constexpr float RB_INF = __builtin_inff();
+
+struct ElemBf {
+  DEV f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  DEV unsigned pack(float lo, float hi) { return pack_bf2(lo, hi); }
+  DEV float lo(unsigned u) { return __uint_as_float(u << 16); }
+  DEV float hi(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+};
+struct ElemHf {
+  DEV f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  DEV unsigned pack(float lo, float hi) {
+    const f32x2_cvt f = {lo, hi};
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(f, f16x2));
+  }
+  DEV float lo(unsigned u) { return (float)__builtin_bit_cast(f16x2, u)[0]; }
+  DEV float hi(unsigned u) { return (float)__builtin_bit_cast(f16x2, u)[1]; }
+};
+
+struct Strides { int64_t b, t, h; };  // elements
+
+struct RbArgs {
+  const uint16_t *q, *k, *v, *o, *dout;
+  Strides sq, sk, sv, so, sdo, sdq, sdk, sdv;
+  const float* table;
+  const int16_t* bucket_of;
+  const int32_t* bucket_range;
+  const int32_t *k_lens, *q_lens, *offsets;
+  uint16_t *out, *dq, *dk, *dv;
+  float *lse, *dtable;
+  const float* lse_in;
+  float *delta, *lse2, *part;  // workspace of the backward
+  int B, Tq, Tk, H, Hk, D, nb, md, causal, offset;
+  float scale, inv_scale, c2;  // c2 = scale * log2(e)
+  int ntile, nblk;             // row tiles per (sequence, head); workgroups
+};
+
+// rows of 2 DP bytes in 16-byte pieces; piece c of row r lies at piece c ^ swz(r).  The key makes both kinds of reads spread over
+// the banks: 16 rows at one piece (ds_read_b128 operands) and 8 rows at four neighbouring pieces (the transposing reads).
+template <int DP>
+DEV int swz(int r) {
+  if constexpr (DP == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+  else if constexpr (DP == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  else return (r >> 2) & 3;
+}
+template <int DP>
+DEV int tile_at(int r, int c) { return r * (2 * DP) + ((c ^ swz<DP>(r)) << 4); }
+
+// the sequence's lengths and query offset; values outside the tensors' extents are cut to them
+struct Seq { int qlen, klen, off; };
+DEV Seq seq_of(const RbArgs& a, int b) {
+  Seq s;
+  s.klen = a.k_lens ? min(max(a.k_lens[b], 0), a.Tk) : a.Tk;
+  s.qlen = a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq;
+  s.off = min(max(a.offsets ? a.offsets[b] : a.offset, -RB_MAX_POS), RB_MAX_POS);
+  return s;
+}
+
+// workgroup -> (sequence, head, row tile): workgroups go to the 8 XCDs in turn; neighbours in (sequence, key head) share K and V
+// and are put on one XCD, so that they meet in its L2
+DEV int xcd_order(int id, int n) {
+  const int x = id & 7, i = id >> 3, full = n >> 3, rest = n & 7;
+  return x * full + min(x, rest) + i;
+}
+
+// table entry -> score units (the products' accumulators hold q . k, scaled later by c2)
+DEV float bias_entry(const RbArgs& a, int r, int h) {
+  const float w = a.table[a.bucket_of[r + a.md] * a.H + h];
+  return w <= -RB_BIG ? -RB_INF : (w > RB_BIG ? RB_BIG : w) * a.inv_scale;
+}
+DEV void spread_table(const RbArgs& a, int h, float* sB, int tid, int nthreads) {
+  const int n = 2 * (a.md + RB_PAD) + 1;
+  for (int i = tid; i < n; i += nthreads) sB[i] = bias_entry(a, min(max(i - a.md - RB_PAD, -a.md), a.md), h);
+}
+
+// over the two half waves (lanes l and l ^ 32), in both
+DEV float half_max(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const unsigned a0 = r[0], a1 = r[1];
+  return fmaxf(__uint_as_float(a0), __uint_as_float(a1));
+}
+DEV float half_sum(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const unsigned a0 = r[0], a1 = r[1];
+  return __uint_as_float(a0) + __uint_as_float(a1);
+}
+
+// ---- 64 rows of a [T, heads, D] tensor on their way to LDS: rows and pieces outside (row >= rows, piece >= D / 8) are zeros
+template <int DP, int NT>
+struct Stage {
+  static constexpr int CPR = DP / 8, N = 64 * CPR / NT;
+  u32x4 r[N];
+  DEV void load(const uint16_t* base, int64_t st, int row0, int rows, int D, int tid, u32x4 (&r)[N]) {
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base + (int64_t)row0 * st), 0, 0x7ffffff0, 0x00020000);
+    const int left = rows - row0;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int x = tid + n * NT, row = x / CPR, c = x % CPR;
+      const bool in = row < left && c * 8 < D;
+      r[n] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, in ? (int)((unsigned)row * (unsigned)st * 2u + c * 16) : -16, 0, 0));
+    }
+  }
+  DEV void store(unsigned char* lds, int tid, const u32x4 (&r)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int x = tid + n * NT, row = x / CPR, c = x % CPR;
+      *reinterpret_cast<u32x4*>(lds + tile_at<DP>(row, c)) = r[n];
+    }
+  }
+};
+
+// one lane's operand fragments of row `row` (piece 2 ks + hi), zeros where the row does not count
+template <int DP>
+DEV void row_frags(const uint16_t* base, int64_t st, int row, bool valid, int D, int hi, u32x4 (&f)[DP / 16]) {
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) {
+    const int c = 2 * ks + hi;
+    f[ks] = u32x4{0, 0, 0, 0};
+    if (valid && c * 8 < D) f[ks] = *reinterpret_cast<const u32x4*>(base + (int64_t)row * st + c * 8);
+  }
+}
+
+// operand fragment of row r of a tile: the 16-byte piece 2 ks + hi
+template <int DP>
+DEV u32x4 frag(const unsigned char* tile, int r, int ks, int hi) {
+  return *reinterpret_cast<const u32x4*>(tile + tile_at<DP>(r, 2 * ks + hi));
+}
+// transposed fragment: rows (= reduction index) kb + 4 hi + 0..3 and kb + 8 + 4 hi + 0..3, column 32 dt + (lane & 31)
+template <int DP>
+DEV u32x4 frag_t(const unsigned char* tile, int kb, int dt, int lane) {
+  const int l16 = lane & 15, hi = lane >> 5;
+  const int r0 = kb + 4 * hi + (l16 >> 2), c = 4 * dt + ((lane >> 4) & 1) * 2 + ((l16 & 3) >> 1), by = (l16 & 1) * 8;
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + tile_at<DP>(r0, c) + by));
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + tile_at<DP>(r0 + 8, c) + by));
+  return __builtin_bit_cast(u32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+template <class E>
+DEV u32x4 pack8(const f32x16& s, int first) {
+  return u32x4{E::pack(s[first], s[first + 1]), E::pack(s[first + 2], s[first + 3]), E::pack(s[first + 4], s[first + 5]),
+               E::pack(s[first + 6], s[first + 7])};
+}
+DEV f32x16 splat16(float x) { return f32x16{x, x, x, x, x, x, x, x, x, x, x, x, x, x, x, x}; }
+
+// four rows' worth of one lane's column: 4 consecutive elements of a row as one 8-byte store
+template <class E>
+DEV void store4(uint16_t* p, float a, float b, float c, float d) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(E::pack(a, b), E::pack(c, d));
+}
+
+// =============================================================================================== forward
+// One workgroup = 4 waves x 32 QW queries of one (sequence, head); 64-key tiles of K and V, double buffered in LDS.
+template <class E, int DP, int QW>
+__global__ __launch_bounds__(256, 2) void rb_fwd_kernel(RbArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  constexpr int P = 2 * DP, TILE = 64 * P, NK = DP / 16, ND = DP / 32;
+  unsigned char* const sK = smem;
+  unsigned char* const sV = smem + 2 * TILE;
+  float* const sB = reinterpret_cast<float*>(smem + 4 * TILE);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, n32 = lane & 31;
+  const int id = xcd_order(blockIdx.x, a.nblk);
+  const int bh = id / a.ntile, tile = a.ntile - 1 - id % a.ntile;  // a causal row's last tiles are the longest: first
+  const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
+  const Seq sq = seq_of(a, b);
+  const int q0 = tile * (128 * QW), p_first = sq.off + q0 + wave * 32 * QW;
+  const uint16_t* const kp = a.k + b * a.sk.b + hk * a.sk.h;
+  const uint16_t* const vp = a.v + b * a.sv.b + hk * a.sv.h;
+
+  int kend = q0 < sq.qlen ? sq.klen : 0, wend = q0 + wave * 32 * QW < sq.qlen ? sq.klen : 0;
+  if (a.causal) {
+    kend = min(kend, sq.off + min(q0 + 128 * QW, sq.qlen));
+    wend = min(wend, p_first + 32 * QW);
+  }
+  const int nt = kend > 0 ? (kend + 63) >> 6 : 0;
+
+  Stage<DP, 256> lk, lv;
+  if (nt > 0) {
+    lk.load(kp, a.sk.t, 0, sq.klen, a.D, tid, lk.r);
+    lv.load(vp, a.sv.t, 0, sq.klen, a.D, tid, lv.r);
+  }
+  u32x4 qf[QW][NK];
+  f32x16 o[QW][ND];
+  float m[QW], l[QW];
+#pragma unroll
+  for (int w = 0; w < QW; ++w) {
+    const int i = q0 + (wave * QW + w) * 32 + n32;
+    row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, i, i < sq.qlen, a.D, hi, qf[w]);
+    m[w] = -RB_INF;
+    l[w] = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[w][d] = splat16(0.f);
+  }
+  spread_table(a, h, sB, tid, 256);
+  if (nt > 0) {
+    lk.store(sK, tid, lk.r);
+    lv.store(sV, tid, lv.r);
+  }
+  __syncthreads();
+  const float left = sB[0], right = sB[2 * (a.md + RB_PAD)];
+
+  for (int t = 0; t < nt; ++t) {
+    const int j0 = t * 64;
+    const bool more = t + 1 < nt;
+    if (more) {
+      lk.load(kp, a.sk.t, j0 + 64, sq.klen, a.D, tid, lk.r);
+      lv.load(vp, a.sv.t, j0 + 64, sq.klen, a.D, tid, lv.r);
+    }
+    const unsigned char* const kt = sK + (t & 1) * TILE;
+    const unsigned char* const vt = sV + (t & 1) * TILE;
+    if (j0 < wend) {
+      f32x16 s[QW][2];
+#pragma unroll
+      for (int w = 0; w < QW; ++w) {
+        const int p0 = p_first + 32 * w;
+        if (j0 - (p0 + 31) >= a.md || j0 + 63 - p0 <= -a.md) {
+          s[w][0] = s[w][1] = splat16(j0 > p0 ? right : left);
+        } else {
+          const float* const bp = sB + (j0 - p0 - n32 + 4 * hi + a.md + RB_PAD);
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[w][u][r] = bp[32 * u + 8 * (r >> 2) + (r & 3)];
+        }
+      }
+#pragma unroll
+      for (int ks = 0; ks < NK; ++ks)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const u32x4 kf = frag<DP>(kt, 32 * u + n32, ks, hi);
+#pragma unroll
+          for (int w = 0; w < QW; ++w) s[w][u] = E::mma(kf, qf[w][ks], s[w][u]);
+        }
+      u32x4 pb[QW][4];
+#pragma unroll
+      for (int w = 0; w < QW; ++w) {
+        const int p0 = p_first + 32 * w;
+        if (j0 + 64 > sq.klen || (a.causal && j0 + 63 > p0)) {
+          const int lim = (a.causal ? min(sq.klen, p0 + n32 + 1) : sq.klen) - j0 - 4 * hi;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (32 * u + 8 * (r >> 2) + (r & 3) >= lim) s[w][u][r] = -RB_INF;
+        }
+        float mx = fmaxf(s[w][0][0], s[w][1][0]);
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(fmaxf(mx, s[w][0][r]), s[w][1][r]);
+        mx = half_max(mx);
+        // the reference moves only when some row's scores outgrow it by 2^8: probabilities stay below 256 and the sums in f32
+        if (__any((mx - m[w]) * a.c2 > 8.f)) {
+          const float up = fmaxf(m[w], mx);
+          const float al = up == -RB_INF ? 1.f : __builtin_amdgcn_exp2f((m[w] - up) * a.c2);
+          m[w] = up;
+          l[w] *= al;
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[w][d][r] *= al;
+        }
+        const float mc = m[w] == -RB_INF ? 0.f : m[w] * a.c2;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            s[w][u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w][u][r], a.c2, -mc));
+            l[w] += s[w][u][r];
+          }
+          pb[w][2 * u] = pack8<E>(s[w][u], 0);
+          pb[w][2 * u + 1] = pack8<E>(s[w][u], 8);
+        }
+      }
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const u32x4 vf = frag_t<DP>(vt, 16 * kk, d, lane);
+#pragma unroll
+          for (int w = 0; w < QW; ++w) o[w][d] = E::mma(vf, pb[w][kk], o[w][d]);
+        }
+    }
+    if (more) {
+      lk.store(sK + ((t + 1) & 1) * TILE, tid, lk.r);
+      lv.store(sV + ((t + 1) & 1) * TILE, tid, lv.r);
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int w = 0; w < QW; ++w) {
+    const int i = q0 + (wave * QW + w) * 32 + n32;
+    if (i >= a.Tq) continue;
+    const float all = half_sum(l[w]);
+    const float sum = i < sq.qlen ? all : 0.f;  // rows behind the sequence and rows without keys: zeros, and -inf
+    const float inv = 1.f / sum;
+    uint16_t* const op = a.out + b * a.so.b + (int64_t)i * a.so.t + h * a.so.h;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = 32 * d + 8 * g + 4 * hi;
+        if (c >= a.D) continue;
+        if (sum == 0.f) store4<E>(op + c, 0.f, 0.f, 0.f, 0.f);
+        else store4<E>(op + c, o[w][d][4 * g] * inv, o[w][d][4 * g + 1] * inv, o[w][d][4 * g + 2] * inv, o[w][d][4 * g + 3] * inv);
+      }
+    if (a.lse != nullptr && hi == 0)
+      a.lse[((int64_t)b * a.H + h) * a.Tq + i] = sum == 0.f ? -RB_INF : (m[w] * a.c2 + __builtin_amdgcn_logf(sum)) * RB_LN2;
+  }
+}
+
+// =============================================================================================== backward
+// delta_i = do_i . o_i and the rows' log-sum-exp in log2 units, +inf where a row has no keys or lies behind its sequence
+// (exp2(s - inf) = 0: such rows drop out of every product).  16 lanes per row.
+template <class E>
+__global__ __launch_bounds__(256) void rb_rows_kernel(RbArgs a) {
+  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), nrow = (int64_t)a.B * a.Tq * a.H;
+  const int c = (threadIdx.x & 15) * 8;
+  if (row >= nrow) return;
+  const int h = (int)(row % a.H);
+  const int64_t bi = row / a.H;
+  const int i = (int)(bi % a.Tq), b = (int)(bi / a.Tq);
+  const Seq sq = seq_of(a, b);
+  float d = 0.f;
+  if (c < a.D && i < sq.qlen) {
+    const u32x4 x = *reinterpret_cast<const u32x4*>(a.dout + b * a.sdo.b + (int64_t)i * a.sdo.t + h * a.sdo.h + c);
+    const u32x4 y = *reinterpret_cast<const u32x4*>(a.o + b * a.so.b + (int64_t)i * a.so.t + h * a.so.h + c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) d += E::lo(x[e]) * E::lo(y[e]) + E::hi(x[e]) * E::hi(y[e]);
+  }
+  d = sum8(d);
+  d += dpp_mov<DPP_MIRROR>(d);
+  if (c == 0) {
+    const int64_t at = ((int64_t)b * a.H + h) * a.Tq + i;
+    const float s = i < sq.qlen ? a.lse_in[at] : -RB_INF;
+    a.delta[at] = d;
+    a.lse2[at] = s == -RB_INF ? RB_INF : s * RB_LOG2E;
+  }
+}
+
+// dq and the table's gradient: 4 waves x 32 queries of one (sequence, head) against 64-key tiles.
+//   S^T = K Q^T (+ bias), dP^T = V dO^T (from -delta), dS = P dP, dQ^T += K^T dS^T
+// The table's gradient is the sum of dS along diagonals.  Far tiles add to one number per lane and side; in near tiles every
+// dS goes to its distance's cell in LDS by ds_add_f32, into a copy per half wave: lanes of one half hold 32 different
+// distances, and the LDS instructions of a wave run in order, so the result does not depend on timing.
+template <class E, int DP>
+__global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  constexpr int P = 2 * DP, TILE = 64 * P, NK = DP / 16, ND = DP / 32;
+  unsigned char* const sK = smem;
+  unsigned char* const sV = smem + 2 * TILE;
+  float* const sB = reinterpret_cast<float*>(smem + 4 * TILE);
+  const int span = 2 * (a.md + RB_PAD) + 1;
+  float* const sG = sB + span;  // [8][span]
+  float* const sFar = sG + 8 * span;  // [4][2]
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, n32 = lane & 31;
+  const int id = xcd_order(blockIdx.x, a.nblk);
+  const int bh = id / a.ntile, tile = a.ntile - 1 - id % a.ntile;
+  const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
+  const Seq sq = seq_of(a, b);
+  const int q0 = tile * 128, i = q0 + wave * 32 + n32, p0 = sq.off + q0 + wave * 32;
+  const uint16_t* const kp = a.k + b * a.sk.b + hk * a.sk.h;
+  const uint16_t* const vp = a.v + b * a.sv.b + hk * a.sv.h;
+  int kend = q0 < sq.qlen ? sq.klen : 0, wend = q0 + wave * 32 < sq.qlen ? sq.klen : 0;
+  if (a.causal) {
+    kend = min(kend, sq.off + min(q0 + 128, sq.qlen));
+    wend = min(wend, p0 + 32);
+  }
+  const int nt = kend > 0 ? (kend + 63) >> 6 : 0;
+
+  Stage<DP, 256> lk, lv;
+  if (nt > 0) {
+    lk.load(kp, a.sk.t, 0, sq.klen, a.D, tid, lk.r);
+    lv.load(vp, a.sv.t, 0, sq.klen, a.D, tid, lv.r);
+  }
+  u32x4 qf[NK], df[NK];
+  row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, i, i < sq.qlen, a.D, hi, qf);
+  row_frags<DP>(a.dout + b * a.sdo.b + h * a.sdo.h, a.sdo.t, i, i < sq.qlen, a.D, hi, df);
+  const int64_t at = ((int64_t)b * a.H + h) * a.Tq + i;
+  const float lse2 = i < a.Tq ? a.lse2[at] : RB_INF, delta = i < a.Tq ? a.delta[at] : 0.f;
+  f32x16 dq[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) dq[d] = splat16(0.f);
+  float farl = 0.f, farr = 0.f;
+  spread_table(a, h, sB, tid, 256);
+  for (int x = tid; x < 8 * span; x += 256) sG[x] = 0.f;
+  if (nt > 0) {
+    lk.store(sK, tid, lk.r);
+    lv.store(sV, tid, lv.r);
+  }
+  __syncthreads();
+  const float left = sB[0], right = sB[span - 1];
+  float* const gp0 = sG + (wave * 2 + hi) * span + (4 * hi - p0 - n32 + a.md + RB_PAD);
+
+  for (int t = 0; t < nt; ++t) {
+    const int j0 = t * 64;
+    const bool more = t + 1 < nt;
+    if (more) {
+      lk.load(kp, a.sk.t, j0 + 64, sq.klen, a.D, tid, lk.r);
+      lv.load(vp, a.sv.t, j0 + 64, sq.klen, a.D, tid, lv.r);
+    }
+    const unsigned char* const kt = sK + (t & 1) * TILE;
+    const unsigned char* const vt = sV + (t & 1) * TILE;
+    if (j0 < wend) {
+      const bool far = j0 - (p0 + 31) >= a.md || j0 + 63 - p0 <= -a.md;
+      const bool edge = j0 + 64 > sq.klen || (a.causal && j0 + 63 > p0);
+      const int lim = (a.causal ? min(sq.klen, p0 + n32 + 1) : sq.klen) - j0 - 4 * hi;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        f32x16 s, dp = splat16(-delta);
+        if (far) {
+          s = splat16(j0 > p0 ? right : left);
+        } else {
+          const float* const bp = sB + (j0 - p0 - n32 + 4 * hi + 32 * u + a.md + RB_PAD);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = bp[8 * (r >> 2) + (r & 3)];
+        }
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) {
+          s = E::mma(frag<DP>(kt, 32 * u + n32, ks, hi), qf[ks], s);
+          dp = E::mma(frag<DP>(vt, 32 * u + n32, ks, hi), df[ks], dp);
+        }
+        if (edge) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (32 * u + 8 * (r >> 2) + (r & 3) >= lim) s[r] = -RB_INF;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, -lse2)) * dp[r];
+        if (far) {
+          float x = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x += s[r];
+          if (j0 > p0) farr += x;
+          else farl += x;
+        } else {
+          float* const gp = gp0 + j0 + 32 * u;
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            __hip_atomic_fetch_add(gp + 8 * (r >> 2) + (r & 3), s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          const u32x4 ds = pack8<E>(s, 8 * kk);
+#pragma unroll
+          for (int d = 0; d < ND; ++d) dq[d] = E::mma(frag_t<DP>(kt, 32 * u + 16 * kk, d, lane), ds, dq[d]);
+        }
+      }
+    }
+    if (more) {
+      lk.store(sK + ((t + 1) & 1) * TILE, tid, lk.r);
+      lv.store(sV + ((t + 1) & 1) * TILE, tid, lv.r);
+    }
+    __syncthreads();
+  }
+
+  if (i < a.Tq) {
+    uint16_t* const op = a.dq + b * a.sdq.b + (int64_t)i * a.sdq.t + h * a.sdq.h;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = 32 * d + 8 * g + 4 * hi;
+        if (c < a.D)
+          store4<E>(op + c, dq[d][4 * g] * a.scale, dq[d][4 * g + 1] * a.scale, dq[d][4 * g + 2] * a.scale, dq[d][4 * g + 3] * a.scale);
+      }
+  }
+  // the workgroup's share of the table's gradient, by distance: copies in order, then what lies beyond the largest distance
+  farl = wave_sum(farl);
+  farr = wave_sum(farr);
+  if (lane == 0) sFar[2 * wave] = farl, sFar[2 * wave + 1] = farr;
+  __syncthreads();
+  for (int x = tid; x < span; x += 256) {
+    float y = 0.f;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) y += sG[c * span + x];
+    sB[x] = y;
+  }
+  __syncthreads();
+  float* const part = a.part + (int64_t)id * (2 * a.md + 1);
+  for (int x = 1 + tid; x < 2 * a.md; x += 256) part[x] = sB[x + RB_PAD];
+  if (wave < 2) {  // the two ends: entries 0 .. PAD and the last PAD + 1
+    float y = 0.f;
+    for (int x = lane; x <= RB_PAD; x += 64) y += sB[wave == 0 ? x : span - 1 - x];
+    y = wave_sum(y);
+    if (lane == 0) part[wave == 0 ? 0 : 2 * a.md] = y + ((sFar[wave] + sFar[2 + wave]) + (sFar[4 + wave] + sFar[6 + wave]));
+  }
+}
+
+// dtable[n, h] = sum over the workgroups of head h and the distances of bucket n, in 64 bits and a fixed order
+__global__ __launch_bounds__(256) void rb_table_kernel(RbArgs a) {
+  __shared__ double red[256];
+  const int n = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
+  const int lo = a.bucket_range[2 * n], width = a.bucket_range[2 * n + 1] - lo;  // distances lo .. lo + width - 1
+  const int64_t total = (int64_t)a.B * a.ntile * width;
+  double s = 0.;
+  for (int64_t x = tid; x < total; x += 256) {
+    const int64_t wg = x / width;
+    const int r = (int)(x % width);
+    const int64_t id = ((wg / a.ntile) * a.H + h) * a.ntile + wg % a.ntile;
+    s += (double)a.part[id * (2 * a.md + 1) + lo + a.md + r];
+  }
+  red[tid] = s;
+  __syncthreads();
+#pragma unroll
+  for (int w = 128; w > 0; w >>= 1) {
+    if (tid < w) red[tid] += red[tid + w];
+    __syncthreads();
+  }
+  if (tid == 0) a.dtable[(int64_t)n * a.H + h] = (float)red[0];
+}
+
+// dk and dv: 4 waves x 32 keys of one (sequence, key head) against 64-query tiles of every head of its group.
+//   S = Q K^T (+ bias), dP = dO V^T (from -delta), dV^T += dO^T P, dK^T += Q^T dS
+template <class E, int DP>
+__global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  constexpr int P = 2 * DP, TILE = 64 * P, NK = DP / 16, ND = DP / 32;
+  unsigned char* const sQ = smem;
+  unsigned char* const sO = smem + 2 * TILE;
+  float* const sL = reinterpret_cast<float*>(smem + 4 * TILE);  // [2][2][64] lse2 | -delta
+  float* const sB = sL + 256;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, n32 = lane & 31;
+  const int id = xcd_order(blockIdx.x, a.nblk);
+  const int bh = id / a.ntile, tile = id % a.ntile;
+  const int b = bh / a.Hk, hk = bh % a.Hk, G = a.H / a.Hk;
+  const Seq sq = seq_of(a, b);
+  const int k0 = tile * 128, j0 = k0 + wave * 32, j = j0 + n32;
+  u32x4 kf[NK], vf[NK];
+  row_frags<DP>(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, j, j < sq.klen, a.D, hi, kf);
+  row_frags<DP>(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, j, j < sq.klen, a.D, hi, vf);
+  f32x16 dk[ND], dv[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) dk[d] = dv[d] = splat16(0.f);
+  // causal: the first query that sees key k0 sits at position k0
+  const int t0 = a.causal ? max(k0 - sq.off, 0) >> 6 : 0;
+  const int t1 = k0 < sq.klen ? (sq.qlen + 63) >> 6 : 0;
+  Stage<DP, 256> lq, lo;
+  float lrow = 0.f;
+
+  for (int g = 0; g < G; ++g) {
+    const int h = hk * G + g;
+    const uint16_t* const qp = a.q + b * a.sq.b + h * a.sq.h;
+    const uint16_t* const dp_ = a.dout + b * a.sdo.b + h * a.sdo.h;
+    const float* const rl = a.lse2 + ((int64_t)b * a.H + h) * a.Tq;
+    const float* const rd = a.delta + ((int64_t)b * a.H + h) * a.Tq;
+    auto load = [&](int t) {
+      lq.load(qp, a.sq.t, t * 64, sq.qlen, a.D, tid, lq.r);
+      lo.load(dp_, a.sdo.t, t * 64, sq.qlen, a.D, tid, lo.r);
+      const int i = t * 64 + lane;
+      if (wave == 0) lrow = i < sq.qlen ? rl[i] : RB_INF;
+      else if (wave == 1) lrow = i < sq.qlen ? -rd[i] : 0.f;
+    };
+    auto store = [&](int buf) {
+      lq.store(sQ + buf * TILE, tid, lq.r);
+      lo.store(sO + buf * TILE, tid, lo.r);
+      if (wave < 2) sL[buf * 128 + wave * 64 + lane] = lrow;
+    };
+    if (t0 < t1) load(t0);
+    __syncthreads();  // the head before has been read
+    spread_table(a, h, sB, tid, 256);
+    if (t0 < t1) store(0);
+    __syncthreads();
+    const float left = sB[0], right = sB[2 * (a.md + RB_PAD)];
+    for (int t = t0; t < t1; ++t) {
+      const int buf = (t - t0) & 1;
+      const bool more = t + 1 < t1;
+      if (more) load(t + 1);
+      const unsigned char* const qt = sQ + buf * TILE;
+      const unsigned char* const ot = sO + buf * TILE;
+      const float* const lt = sL + buf * 128;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int p0 = sq.off + t * 64 + 32 * u;  // position of the sub-tile's first query
+        if (j0 >= sq.klen || (a.causal && j0 > p0 + 31)) continue;
+        f32x16 s, dp;
+        if (j0 - (p0 + 31) >= a.md || j0 + 31 - p0 <= -a.md) {
+          s = splat16(j0 > p0 ? right : left);
+        } else {
+          const float* const bp = sB + (j - p0 - 4 * hi + a.md + RB_PAD);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = bp[-(8 * (r >> 2) + (r & 3))];
+        }
+        float ls[16];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(lt + 32 * u + 8 * q + 4 * hi);
+          const f32x4 y = *reinterpret_cast<const f32x4*>(lt + 64 + 32 * u + 8 * q + 4 * hi);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) ls[4 * q + r] = x[r], dp[4 * q + r] = y[r];
+        }
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) {
+          s = E::mma(frag<DP>(qt, 32 * u + n32, ks, hi), kf[ks], s);
+          dp = E::mma(frag<DP>(ot, 32 * u + n32, ks, hi), vf[ks], dp);
+        }
+        if (a.causal && j0 + 31 > p0) {
+          const int lim = j - p0 - 4 * hi;  // queries before it do not see the key
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (8 * (r >> 2) + (r & 3) < lim) s[r] = -RB_INF;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, -ls[r]));
+          dp[r] *= s[r];
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          const u32x4 pb = pack8<E>(s, 8 * kk), db = pack8<E>(dp, 8 * kk);
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            dv[d] = E::mma(frag_t<DP>(ot, 32 * u + 16 * kk, d, lane), pb, dv[d]);
+            dk[d] = E::mma(frag_t<DP>(qt, 32 * u + 16 * kk, d, lane), db, dk[d]);
+          }
+        }
+      }
+      if (more) store(buf ^ 1);
+      __syncthreads();
+    }
+  }
+  if (j >= a.Tk) return;
+  const bool in = j < sq.klen;  // rows behind the sequence get zeros
+  uint16_t* const kp = a.dk + b * a.sdk.b + (int64_t)j * a.sdk.t + hk * a.sdk.h;
+  uint16_t* const vp = a.dv + b * a.sdv.b + (int64_t)j * a.sdv.t + hk * a.sdv.h;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * d + 8 * g + 4 * hi;
+      if (c >= a.D) continue;
+      float x[8];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = in ? dk[d][4 * g + r] * a.scale : 0.f, x[4 + r] = in ? dv[d][4 * g + r] : 0.f;
+      store4<E>(kp + c, x[0], x[1], x[2], x[3]);
+      store4<E>(vp + c, x[4], x[5], x[6], x[7]);
+    }
+}
+
+// =============================================================================================== host side
+bool strides_ok(const int64_t* s) {
+  // 16-byte rows; a tile of 64 rows must stay within a 31-bit byte offset
+  return s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0 && s[1] >= 0 && s[1] < (1 << 23) && s[0] >= 0 && s[2] >= 0;
+}
+Strides to_strides(const int64_t* s) { return Strides{s[0], s[1], s[2]}; }
+
+int check_args(const csship_relbias* p) {
+  if (p == nullptr) return CSSHIP_ENULL;
+  if (p->B < 0 || p->Tq < 0 || p->Tk < 0 || p->H < 1 || p->Hk < 1 || p->H % p->Hk != 0) return CSSHIP_EBADSHAPE;
+  if (p->Tq > RB_MAX_POS || p->Tk > RB_MAX_POS) return CSSHIP_EBADSHAPE;
+  if ((int64_t)p->B * p->H * ((int64_t)(p->Tq > p->Tk ? p->Tq : p->Tk) + 128) > 0x7fffffff) return CSSHIP_EBADSHAPE;
+  if (p->D < 8 || p->D > 128 || p->D % 8 != 0) return CSSHIP_EUNSUPPORTED;
+  if (p->dtype != CSSHIP_RELBIAS_BF16 && p->dtype != CSSHIP_RELBIAS_FP16) return CSSHIP_EUNSUPPORTED;
+  if (p->n_buckets < 2 || p->n_buckets > 32767 || p->max_distance < 1 || p->max_distance > CSSHIP_RELBIAS_MAX_DISTANCE)
+    return CSSHIP_EUNSUPPORTED;
+  if (!(p->scale > 1e-6f && p->scale < 1e6f)) return CSSHIP_EUNSUPPORTED;
+  if (p->table == nullptr || p->bucket_of == nullptr) return CSSHIP_ENULL;
+  const bool rows = p->B > 0 && p->Tq > 0, keys = p->B > 0 && p->Tk > 0;
+  if ((rows && p->q == nullptr) || (keys && (p->k == nullptr || p->v == nullptr))) return CSSHIP_ENULL;
+  if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v)) return CSSHIP_EALIGN;
+  if (!strides_ok(p->q_stride) || !strides_ok(p->k_stride) || !strides_ok(p->v_stride)) return CSSHIP_EALIGN;
+  return CSSHIP_OK;
+}
+
+RbArgs to_args(const csship_relbias* p) {
+  RbArgs a{};
+  a.q = p->q; a.k = p->k; a.v = p->v;
+  a.sq = to_strides(p->q_stride); a.sk = to_strides(p->k_stride); a.sv = to_strides(p->v_stride);
+  a.table = p->table; a.bucket_of = p->bucket_of; a.bucket_range = p->bucket_range;
+  a.k_lens = p->k_lens; a.q_lens = p->q_lens; a.offsets = p->offsets;
+  a.B = p->B; a.Tq = p->Tq; a.Tk = p->Tk; a.H = p->H; a.Hk = p->Hk; a.D = p->D;
+  a.nb = p->n_buckets; a.md = p->max_distance; a.causal = p->causal != 0; a.offset = p->offset;
+  a.scale = p->scale; a.inv_scale = 1.f / p->scale; a.c2 = p->scale * RB_LOG2E;
+  return a;
+}
+
+size_t fwd_lds(int DP, int md) { return (size_t)4 * 64 * 2 * DP + (2 * (md + RB_PAD) + 1) * 4; }
+size_t dq_lds(int DP, int md) { return (size_t)4 * 64 * 2 * DP + (size_t)9 * (2 * (md + RB_PAD) + 1) * 4 + 32; }
+size_t dkv_lds(int DP, int md) { return fwd_lds(DP, md) + 1024; }
+
+// launches with more than 64 KB of LDS have to be allowed, per device: asked for at each such launch
+template <class K>
+int launch(K kernel, int64_t blocks, size_t lds, const RbArgs& a, hipStream_t s) {
+  if (lds > 64 * 1024 &&
+      hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
+    return CSSHIP_ELAUNCH;
+  kernel<<<(unsigned)blocks, 256, lds, s>>>(a);
+  CSSHIP_CHECK_LAUNCH();
+  return CSSHIP_OK;
+}
+
+template <class E, int DP>
+int launch_fwd(RbArgs a, hipStream_t s) {
+  a.ntile = (a.Tq + 127) / 128;
+  a.nblk = a.B * a.H * a.ntile;
+  if (a.nblk == 0) return CSSHIP_OK;
+  return launch(rb_fwd_kernel<E, DP, 1>, a.nblk, fwd_lds(DP, a.md), a, s);
+}
+
+template <class E, int DP>
+int launch_bwd(RbArgs a, hipStream_t s) {
+  const int64_t rows = (int64_t)a.B * a.Tq * a.H;
+  if (rows > 0)
+    if (const int rc = launch(rb_rows_kernel<E>, (rows + 15) / 16, 0, a, s)) return rc;
+  RbArgs d = a;
+  d.ntile = (a.Tq + 127) / 128;
+  d.nblk = a.B * a.H * d.ntile;
+  if (d.nblk > 0)
+    if (const int rc = launch(rb_dq_kernel<E, DP>, d.nblk, dq_lds(DP, a.md), d, s)) return rc;
+  RbArgs e = a;
+  e.ntile = (a.Tk + 127) / 128;
+  e.nblk = a.B * a.Hk * e.ntile;
+  if (e.nblk > 0)
+    if (const int rc = launch(rb_dkv_kernel<E, DP>, e.nblk, dkv_lds(DP, a.md), e, s)) return rc;
+  rb_table_kernel<<<dim3(a.nb, a.H), 256, 0, s>>>(d);
+  CSSHIP_CHECK_LAUNCH();
+  return CSSHIP_OK;
+}
+
+template <class E>
+int by_width(const RbArgs& a, bool bwd, hipStream_t s) {
+  if (a.D <= 32) return bwd ? launch_bwd<E, 32>(a, s) : launch_fwd<E, 32>(a, s);
+  if (a.D <= 64) return bwd ? launch_bwd<E, 64>(a, s) : launch_fwd<E, 64>(a, s);
+  return bwd ? launch_bwd<E, 128>(a, s) : launch_fwd<E, 128>(a, s);
+}
+
+int64_t row_words(const csship_relbias* p) { return ((int64_t)p->B * p->H * p->Tq + 3) / 4 * 4; }
+
+}  // namespace
+
+extern "C" {
+
+size_t csship_relbias_fwd_workspace(const csship_relbias* p) {
+  (void)p;
+  return 0;
+}
+
+int csship_relbias_fwd(const csship_relbias* p, uint16_t* out, const int64_t* out_stride, float* lse, void* workspace,
+                       size_t workspace_bytes, csship_stream_t stream) {
+  if (const int rc = check_args(p)) return rc;
+  (void)workspace;
+  if (workspace_bytes < csship_relbias_fwd_workspace(p)) return CSSHIP_EWORKSPACE;
+  if (p->B == 0 || p->Tq == 0) return CSSHIP_OK;
+  if (out == nullptr || out_stride == nullptr) return CSSHIP_ENULL;
+  if (!aligned8(out) || !strides_ok(out_stride)) return CSSHIP_EALIGN;
+  RbArgs a = to_args(p);
+  a.out = out;
+  a.so = to_strides(out_stride);
+  a.lse = lse;
+  return p->dtype == CSSHIP_RELBIAS_BF16 ? by_width<ElemBf>(a, false, as_stream(stream)) : by_width<ElemHf>(a, false, as_stream(stream));
+}
+
+size_t csship_relbias_bwd_workspace(const csship_relbias* p) {
+  if (check_args(p) != CSSHIP_OK) return 0;
+  const int64_t wgs = (int64_t)p->B * p->H * ((p->Tq + 127) / 128);
+  return (size_t)(2 * row_words(p) + wgs * (2 * p->max_distance + 1)) * 4 + 16;
+}
+
+int csship_relbias_bwd(const csship_relbias* p, const uint16_t* out, const int64_t* out_stride, const float* lse, const uint16_t* dout,
+                       const int64_t* dout_stride, uint16_t* dq, const int64_t* dq_stride, uint16_t* dk, const int64_t* dk_stride,
+                       uint16_t* dv, const int64_t* dv_stride, float* dtable, void* workspace, size_t workspace_bytes,
+                       csship_stream_t stream) {
+  if (const int rc = check_args(p)) return rc;
+  const bool rows = p->B > 0 && p->Tq > 0, keys = p->B > 0 && p->Tk > 0;
+  if (p->bucket_range == nullptr || dtable == nullptr || out_stride == nullptr || dout_stride == nullptr || dq_stride == nullptr ||
+      dk_stride == nullptr || dv_stride == nullptr || workspace == nullptr)
+    return CSSHIP_ENULL;
+  if ((rows && (out == nullptr || lse == nullptr || dout == nullptr || dq == nullptr)) || (keys && (dk == nullptr || dv == nullptr)))
+    return CSSHIP_ENULL;
+  if (!aligned16(out) || !aligned16(dout) || !aligned8(dq) || !aligned8(dk) || !aligned8(dv) || !aligned16(workspace)) return CSSHIP_EALIGN;
+  if (!strides_ok(out_stride) || !strides_ok(dout_stride) || !strides_ok(dq_stride) || !strides_ok(dk_stride) || !strides_ok(dv_stride))
+    return CSSHIP_EALIGN;
+  if (workspace_bytes < csship_relbias_bwd_workspace(p)) return CSSHIP_EWORKSPACE;
+  RbArgs a = to_args(p);
+  a.o = out; a.so = to_strides(out_stride);
+  a.dout = dout; a.sdo = to_strides(dout_stride);
+  a.lse_in = lse;
+  a.dq = dq; a.sdq = to_strides(dq_stride);
+  a.dk = dk; a.sdk = to_strides(dk_stride);
+  a.dv = dv; a.sdv = to_strides(dv_stride);
+  a.dtable = dtable;
+  a.delta = static_cast<float*>(workspace);
+  a.lse2 = a.delta + row_words(p);
+  a.part = a.lse2 + row_words(p);
+  return p->dtype == CSSHIP_RELBIAS_BF16 ? by_width<ElemBf>(a, true, as_stream(stream)) : by_width<ElemHf>(a, true, as_stream(stream));
+}
+
+}  // extern "C"

@@ -271,6 +271,140 @@ def mha_relpos_probs(qkv, pe_pack, lse, n_head, drop=None):
     return p if drop is None else (p, pd)
 
 
+# ---------------------------------------------------------------- attention with a bucketed relative-position bias
+def relbias_bucket_map(n_buckets, max_distance, two_sided=True):
+    """The bucket of every distance r = key position - query position in -max_distance .. max_distance (a list of 2 *
+    max_distance + 1; further distances take the end entries).  Two-sided: the upper half of the buckets serves r > 0, each
+    side has nb = n_buckets / 2 by |r|; one-sided: nb = n_buckets by max(-r, 0).  The first e = nb // 2 distances have a
+    bucket each, the others share min(nb - 1, e + floor((nb - e) log(d / e) / log(max_distance / e))); the borders are
+    decided in whole numbers: d is in bucket e + t or above iff (d / e)^(nb - e) >= (max_distance / e)^t."""
+    n_buckets, max_distance = int(n_buckets), int(max_distance)
+    if two_sided and n_buckets % 2:
+        raise RuntimeError("css_amd: a two-sided bucket map needs an even number of buckets")
+    nb = n_buckets // 2 if two_sided else n_buckets
+    e = nb // 2
+    if e < 1 or not e < max_distance <= _lib.RELBIAS_MAX_DISTANCE:
+        raise RuntimeError(f"css_amd: {n_buckets} buckets up to distance {max_distance}: at least 2 buckets a side, and a largest "
+                           f"distance above half of a side's buckets and up to {_lib.RELBIAS_MAX_DISTANCE}")
+    side, t, power = [], 0, nb - e
+    for d in range(max_distance + 1):
+        if d < e:
+            side.append(d)
+            continue
+        while t + 1 < power and d ** power * e ** (t + 1) >= e ** power * max_distance ** (t + 1):
+            t += 1
+        side.append(e + t)
+    back = [side[-r] for r in range(-max_distance, 1)]
+    return back + ([nb + d for d in side[1:]] if two_sided else [0] * max_distance)
+
+
+_RELBIAS_BUCKETS = {}  # (device index, n_buckets, max_distance, two_sided) -> (bucket_of, bucket_range); kept: a captured graph reads them
+
+
+def relbias_buckets(buckets, device):
+    """(bucket_of int16, bucket_range int32 [n, 2]) of csship_relbias on ``device`` for buckets = (n_buckets, max_distance[,
+    two_sided]).  Built at the first call with these settings, which therefore must not be under graph capture."""
+    n, far, two = (*buckets, True)[:3]
+    key = (device.index, int(n), int(far), bool(two))
+    got = _RELBIAS_BUCKETS.get(key)
+    if got is None:
+        m = relbias_bucket_map(n, far, two)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("css_amd: first use of these bucket settings under graph capture: call ops.relbias_buckets before it")
+        # distances in order: a bucket's distances are contiguous, except that the one-sided map gives bucket 0 to all r >= 0
+        rng = [[0, 0] for _ in range(key[1])]
+        for i, b in enumerate(m):
+            r = i - key[2]
+            rng[b] = [r if rng[b][0] == rng[b][1] else rng[b][0], r + 1]
+        got = _RELBIAS_BUCKETS[key] = (torch.tensor(m, dtype=torch.int16).to(device), torch.tensor(rng, dtype=torch.int32).to(device))
+    return got
+
+
+def _relbias_rows(t, name, like=None):
+    """A [B, T, heads, D] operand whose rows csship_relbias can address (a copy where its strides do not allow it)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"css_amd: '{name}' must be a CUDA/HIP tensor (no CPU path exists)")
+    if t.dim() != 4:
+        raise RuntimeError(f"css_amd: '{name}' must be [batch, frames, heads, width], got {tuple(t.shape)}")
+    if t.dtype not in (torch.bfloat16, torch.float16) or (like is not None and t.dtype != like.dtype):
+        raise TypeError(f"css_amd: '{name}' must be {'bfloat16 or float16' if like is None else like.dtype}, got {t.dtype}")
+    if like is not None and t.device != like.device:
+        raise RuntimeError(f"css_amd: '{name}' is on {t.device}, the queries on {like.device}")
+    s = t.stride()
+    if s[3] != 1 or (s[0] | s[1] | s[2]) & 7 or s[1] >= 1 << 23 or t.data_ptr() & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _relbias_struct(q, k, v, table, buckets, scale, causal, offset, k_lens, q_lens):
+    """Checks the operands of csship_relbias and fills its struct; returns (struct, tensors it points to)."""
+    q = _relbias_rows(q, "q")
+    k, v = _relbias_rows(k, "k", q), _relbias_rows(v, "v", q)
+    B, Tq, H, D = q.shape
+    Tk, Hk = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise RuntimeError(f"css_amd: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not belong together")
+    if Hk < 1 or H < 1 or H % Hk:
+        raise RuntimeError(f"css_amd: {H} query heads cannot share {Hk} key heads evenly")
+    if D % 8 or not 8 <= D <= 128:
+        raise RuntimeError(f"css_amd: head width {D}: a multiple of 8 up to 128")
+    _need(table, torch.float32, "table")
+    n, far = int(buckets[0]), int(buckets[1])
+    if tuple(table.shape) != (n, H) or table.device != q.device:
+        raise RuntimeError(f"css_amd: 'table' must be [{n}, {H}] on {q.device}, got {tuple(table.shape)} on {table.device}")
+    table = table.detach().contiguous()
+    for name, x in (("k_lens", k_lens), ("q_lens", q_lens), ("offset", offset)):
+        if isinstance(x, torch.Tensor):
+            if x.dtype != torch.int32 or tuple(x.shape) != (B,) or x.device != q.device or not x.is_contiguous():
+                raise RuntimeError(f"css_amd: '{name}' must be a dense int32 [{B}] on {q.device}")
+        elif x is not None and name != "offset":
+            raise TypeError(f"css_amd: '{name}' must be an int32 tensor or None")
+    each = isinstance(offset, torch.Tensor)
+    if not each and not -(1 << 28) <= int(offset) <= 1 << 28:
+        raise RuntimeError(f"css_amd: offset {offset} out of range")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 1e-6 < scale < 1e6:
+        raise RuntimeError(f"css_amd: scale {scale}: a positive number of ordinary size")
+    bucket_of, bucket_range = relbias_buckets(buckets, q.device)
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    p = _lib.RelBias(q.data_ptr(), k.data_ptr(), v.data_ptr(), sq[:3], sk[:3], sv[:3], table.data_ptr(), bucket_of.data_ptr(),
+                     bucket_range.data_ptr(), k_lens.data_ptr() if k_lens is not None else None,
+                     q_lens.data_ptr() if q_lens is not None else None, offset.data_ptr() if each else None,
+                     _lib.RELBIAS_BF16 if q.dtype == torch.bfloat16 else _lib.RELBIAS_FP16, B, Tq, Tk, H, Hk, D, n, far,
+                     1 if causal else 0, 0 if each else int(offset), scale)
+    return p, (q, k, v, table)
+
+
+def _strides3(t):
+    return _lib._s3(*t.stride()[:3])
+
+
+def mha_relbias(q, k, v, table, buckets, *, scale=None, causal=False, offset=0, k_lens=None, q_lens=None, want_lse=False):
+    """Attention with a learned bias per bucket of the key-query distance (csship_relbias_fwd; formulas in include/csship.h).
+
+    q [B,Tq,H,D], k / v [B,Tk,Hk,D] bf16 or fp16, Hk dividing H (grouped heads), D a multiple of 8 up to 128; strided views (a
+    packed q|k|v projection, a cache) are read in place.  table f32 [n_buckets, H]; buckets = (n_buckets, max_distance[,
+    two_sided=True]).  scale: D ** -0.5 unless given.  Query i sits at position i + offset, key j at j (offset: a number or int32
+    [B] on the device; streaming: frames kept so far); causal: keys behind the query's position are not seen.  k_lens / q_lens
+    int32 [B]: lengths of a padded batch; what lies behind them is not read, and those rows of the result are zeros.
+    A query without keys gets zeros (log-sum-exp -inf).  -> out [B,Tq,H,D], or (out, lse f32 [B,H,Tq]) with want_lse."""
+    p, keep = _relbias_struct(q, k, v, table, buckets, scale, causal, offset, k_lens, q_lens)
+    q = keep[0]
+    if q.device.index != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return mha_relbias(q, k, v, table, buckets, scale=scale, causal=causal, offset=offset, k_lens=k_lens, q_lens=q_lens,
+                               want_lse=want_lse)
+    B, Tq, H, D = q.shape
+    out = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, Tq), dtype=torch.float32, device=q.device) if want_lse else None
+    h = lib()
+    n = h.csship_relbias_fwd_workspace(C.byref(p))
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+    check(h.csship_relbias_fwd(C.byref(p), out.data_ptr(), _strides3(out), lse.data_ptr() if want_lse else None,
+                               ws.data_ptr() if n else None, n, torch.cuda.current_stream().cuda_stream))
+    return (out, lse) if want_lse else out
+
+
 def conv_weights_struct(t):
     """t: dict of f32 CUDA tensors keyed like _lib.ConvWeights fields."""
     cw = _lib.ConvWeights()

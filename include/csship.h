@@ -1139,6 +1139,49 @@ int csship_debug_timeline_read(int tag, double* total_ms, int* count);
 void csship_debug_timeline_calibrate(csship_stream_t stream, int pairs);
 void csship_debug_stamps(void* device_buffer);
 
+/* ---- attention with a bucketed relative-position bias (css_amd/csrc/relbias.hip)
+ * Query i of sequence b sits at position p = i + offset_b, key j at position j; r = j - p; query head h reads key head
+ * h / (H / Hk).  Query i sees key j iff i < q_len_b, j < k_len_b and, with `causal`, r <= 0.
+ *   s_ij   = scale q_i . k_j + table[bucket(r), h]
+ *   lse_i  = log sum_j exp(s_ij),  P_ij = exp(s_ij - lse_i),  out_i = sum_j P_ij v_j     (no key: out 0, lse -inf)
+ *   delta_i = dout_i . out_i,  dS_ij = P_ij (dout_i . v_j - delta_i)
+ *   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,  dv_j = sum_i P_ij dout_i  (sums over the heads of the group),
+ *   dtable[n, h] = sum of dS_ij over the pairs with bucket(r) = n, over all sequences
+ * q, out, dout, dq [B, Tq, H, D]; k, v, dk, dv [B, Tk, Hk, D], bf16 or fp16 (dtype), strides in ELEMENTS for (sequence, frame,
+ * head), the last dimension dense; strides are non-negative multiples of 8, the frame stride below 2^23, inputs 16-byte and
+ * results 8-byte aligned.  D is a multiple of 8 up to 128.  lse f32 [B, H, Tq] dense.  table, dtable f32 [n_buckets, H] dense.
+ * bucket_of int16 [2 max_distance + 1]: the bucket of r at bucket_of[r + max_distance]; distances beyond +-max_distance take the
+ * end entries.  bucket_range int32 [n_buckets][2] (backward): bucket n holds the distances bucket_range[n][0] <= r <
+ * bucket_range[n][1] of those 2 max_distance + 1 (equal bounds: none); a bucket's distances have to be contiguous.
+ * k_lens / q_lens int32 [B] or NULL (all Tk / Tq); values are cut to 0 .. Tk / Tq.  offsets int32 [B], or NULL: `offset` for
+ * all; cut to +-2^28.  What lies behind a sequence's end in q, k, v, out, dout is never read into a result: it may hold
+ * anything; results there are zeros (lse -inf).  A key that is only masked by `causal` must hold finite values.
+ * A table entry of -2^20 or less bans its distances (the pairs drop out, their gradient is 0); one above 2^20 counts as 2^20.
+ * Every sum is in a fixed order: results do not change from run to run. */
+#define CSSHIP_RELBIAS_BF16 0
+#define CSSHIP_RELBIAS_FP16 1
+#define CSSHIP_RELBIAS_MAX_DISTANCE 1024
+typedef struct {
+  const uint16_t *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const float* table;
+  const int16_t* bucket_of;
+  const int32_t* bucket_range;
+  const int32_t *k_lens, *q_lens, *offsets;
+  int32_t dtype, B, Tq, Tk, H, Hk, D, n_buckets, max_distance, causal, offset;
+  float scale;
+} csship_relbias;
+/* out and, unless NULL, lse.  workspace may be NULL where csship_relbias_fwd_workspace is 0. */
+size_t csship_relbias_fwd_workspace(const csship_relbias* p);
+int csship_relbias_fwd(const csship_relbias* p, uint16_t* out, const int64_t* out_stride, float* lse, void* workspace,
+                       size_t workspace_bytes, csship_stream_t stream);
+/* The probabilities are recomputed from q, k, table and the forward's lse; no T x T operand exists in memory. */
+size_t csship_relbias_bwd_workspace(const csship_relbias* p);
+int csship_relbias_bwd(const csship_relbias* p, const uint16_t* out, const int64_t* out_stride, const float* lse, const uint16_t* dout,
+                       const int64_t* dout_stride, uint16_t* dq, const int64_t* dq_stride, uint16_t* dk, const int64_t* dk_stride,
+                       uint16_t* dv, const int64_t* dv_stride, float* dtable, void* workspace, size_t workspace_bytes,
+                       csship_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
