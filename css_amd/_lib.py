@@ -6,6 +6,7 @@ every op wrapper refuses non-CUDA tensors.  Build it with ``make -C css_amd/csrc
 """
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "csrc", "libcsship.so")
@@ -81,16 +82,11 @@ class BgemmParams(C.Structure):
                 ("sX1", _i64), ("sX2", _i64), ("alpha", _f32), ("band", _i32), ("band_stride", _i32)]
 
 
-_s3 = C.c_int64 * 3
-
-
-class RelBias(C.Structure):  # csship_relbias
-    _fields_ = [("q", _p), ("k", _p), ("v", _p), ("q_stride", _s3), ("k_stride", _s3), ("v_stride", _s3),
-                ("table", _p), ("bucket_of", _p), ("bucket_range", _p), ("k_lens", _p), ("q_lens", _p), ("offsets", _p),
-                ("dtype", _i32), ("B", _i32), ("Tq", _i32), ("Tk", _i32), ("H", _i32), ("Hk", _i32), ("D", _i32),
-                ("n_buckets", _i32), ("max_distance", _i32), ("causal", _i32), ("offset", _i32), ("scale", _f32)]
-
-
+# csship_relbias, packed straight into bytes (filling a ctypes structure field by field costs several microseconds a call):
+# q k v | q_stride k_stride v_stride | table bucket_of bucket_range k_lens q_lens offsets | dtype B Tq Tk H Hk D n_buckets
+# max_distance causal offset | scale
+RELBIAS = struct.Struct("@3Q9q6Q11if")
+STRIDE3 = struct.Struct("@3q")
 RELBIAS_BF16, RELBIAS_FP16, RELBIAS_MAX_DISTANCE = 0, 1, 1024
 _dc = C.POINTER(DropoutCfg)
 
@@ -267,10 +263,10 @@ SIGNATURES = {
     "csship_attn_pos_bwd_ds_parts": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i32, _p, _p, _i32, _i32, _i32, _i32, _p, _sz, _p]),
     "csship_mha_relpos_bwd_fused_parts": (_i32, [_i32, _i32, _i32]),
     "csship_mha_relpos_bwd_fused": (_i32, [_p, _p, _i32, _i32, _p, _p, _p, _p, _i64, _p, _p, _i32, _i32, _i32, _dc, _p]),
-    "csship_relbias_fwd_workspace": (_sz, [C.POINTER(RelBias)]),
-    "csship_relbias_fwd": (_i32, [C.POINTER(RelBias), _p, _s3, _p, _p, _sz, _p]),
-    "csship_relbias_bwd_workspace": (_sz, [C.POINTER(RelBias)]),
-    "csship_relbias_bwd": (_i32, [C.POINTER(RelBias), _p, _s3, _p, _p, _s3, _p, _s3, _p, _s3, _p, _s3, _p, _p, _sz, _p]),
+    "csship_relbias_fwd_workspace": (_sz, [_p]),
+    "csship_relbias_fwd": (_i32, [_p, _p, _p, _p, _p, _sz, _p]),
+    "csship_relbias_bwd_workspace": (_sz, [_p]),
+    "csship_relbias_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
     "csship_debug_timeline": (None, [_i32]),
     "csship_debug_timeline_read": (_i32, [_i32, C.POINTER(C.c_double), C.POINTER(_i32)]),
     "csship_debug_timeline_calibrate": (None, [_p, _i32]),

@@ -60,10 +60,10 @@ struct RbArgs {
   uint16_t *out, *dq, *dk, *dv;
   float *lse, *dtable;
   const float* lse_in;
-  float *delta, *lse2, *part;  // workspace of the backward
+  float *delta, *lse2, *part;  // workspace
   int B, Tq, Tk, H, Hk, D, nb, md, causal, offset;
   float scale, inv_scale, c2;  // c2 = scale * log2(e)
-  int ntile, nblk;             // row tiles per (sequence, head); workgroups
+  int ntile, nblk, nsplit, nqtile;     // row tiles per (sequence, head); workgroups; key ranges (rb_few_kernel)
 };
 
 // rows of 2 DP bytes in 16-byte pieces; piece c of row r lies at piece c ^ swz(r).  The key makes both kinds of reads spread over
@@ -339,50 +339,257 @@ __global__ __launch_bounds__(256, 2) void rb_fwd_kernel(RbArgs a) {
   }
 }
 
-// =============================================================================================== backward
-// delta_i = do_i . o_i and the rows' log-sum-exp in log2 units, +inf where a row has no keys or lies behind its sequence
-// (exp2(s - inf) = 0: such rows drop out of every product).  16 lanes per row.
-template <class E>
-__global__ __launch_bounds__(256) void rb_rows_kernel(RbArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), nrow = (int64_t)a.B * a.Tq * a.H;
-  const int c = (threadIdx.x & 15) * 8;
-  if (row >= nrow) return;
-  const int h = (int)(row % a.H);
-  const int64_t bi = row / a.H;
-  const int i = (int)(bi % a.Tq), b = (int)(bi / a.Tq);
+// ------------------------------------------------------------------------------------ forward, few query rows
+// Rows = (query, head of the group) of one (sequence, key head), 32 to a workgroup: a head's group shares the K and V it reads.
+// Nothing is reused across waves, so each of the 4 waves streams its own 32-key tiles (every fourth of the workgroup's), K straight
+// into operand registers, V through a wave's own LDS tile for the transposing reads, the next tile's loads in flight; the waves'
+// running softmax states are joined in LDS.  Bound by the bytes of K and V.  Where few workgroups would run, the keys are split
+// over `nsplit` of them: states go to the workspace and rb_join_kernel joins them in order.
+template <class E, int DP>
+__global__ __launch_bounds__(256, 2) void rb_few_kernel(RbArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  constexpr int P = 2 * DP, NK = DP / 16, ND = DP / 32, CPR = DP / 8, RPI = 64 / CPR, NV = 32 / RPI;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, n32 = lane & 31;
+  unsigned char* const sV = smem + wave * 32 * P;
+  const int G = a.H / a.Hk, R = a.Tq * G;
+  const int id = xcd_order(blockIdx.x, a.nblk);
+  const int split = id % a.nsplit, rb = id / a.nsplit % a.ntile, bk = id / a.nsplit / a.ntile;
+  const int b = bk / a.Hk, hk = bk % a.Hk;
   const Seq sq = seq_of(a, b);
-  float d = 0.f;
-  if (c < a.D && i < sq.qlen) {
-    const u32x4 x = *reinterpret_cast<const u32x4*>(a.dout + b * a.sdo.b + (int64_t)i * a.sdo.t + h * a.sdo.h + c);
-    const u32x4 y = *reinterpret_cast<const u32x4*>(a.o + b * a.so.b + (int64_t)i * a.so.t + h * a.so.h + c);
+  const int row = rb * 32 + n32, i = row / G, h = hk * G + row % G;
+  const bool valid = row < R && i < sq.qlen;
+  const int p = sq.off + i, i_last = min((rb * 32 + 31) / G, sq.qlen - 1);
+  int kend = rb * 32 / G < sq.qlen ? sq.klen : 0;
+  if (a.causal) kend = min(kend, sq.off + i_last + 1);
+  const int ntile = kend > 0 ? (kend + 31) >> 5 : 0, per = (ntile + a.nsplit - 1) / a.nsplit;
+  const int t1 = min(ntile, (split + 1) * per);
+  const uint16_t* const kp = a.k + b * a.sk.b + hk * a.sk.h;
+  const uint16_t* const vp = a.v + b * a.sv.b + hk * a.sv.h;
+
+  u32x4 qf[NK], kf[NK], vr[NV];
+  row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, i, valid, a.D, hi, qf);
+  const int hc = min(h, a.H - 1);
+  const float left = bias_entry(a, -a.md, hc), right = bias_entry(a, a.md, hc);
+  auto load = [&](int t) {
+    const int j0 = t * 32, left_rows = sq.klen - j0;
+    const __amdgpu_buffer_rsrc_t rk =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(kp + (int64_t)j0 * a.sk.t), 0, 0x7ffffff0, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rv =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(vp + (int64_t)j0 * a.sv.t), 0, 0x7ffffff0, 0x00020000);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) d += E::lo(x[e]) * E::lo(y[e]) + E::hi(x[e]) * E::hi(y[e]);
+    for (int ks = 0; ks < NK; ++ks) {
+      const int c = 2 * ks + hi;
+      kf[ks] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                             rk, n32 < left_rows && c * 8 < a.D ? (int)((unsigned)n32 * (unsigned)a.sk.t * 2u + c * 16) : -16, 0, 0));
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int r = n * RPI + lane / CPR, c = lane % CPR;
+      vr[n] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                            rv, r < left_rows && c * 8 < a.D ? (int)((unsigned)r * (unsigned)a.sv.t * 2u + c * 16) : -16, 0, 0));
+    }
+  };
+  f32x16 o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) o[d] = splat16(0.f);
+  float m = -RB_INF, l = 0.f;
+  int t = __builtin_amdgcn_readfirstlane(split * per + wave);
+  if (t < t1) load(t);
+  const int p_lo = sq.off + rb * 32 / G, p_hi = sq.off + (rb * 32 + 31) / G;  // positions of the workgroup's rows
+  for (; t < t1; t += 4) {
+    const int j0 = t * 32;
+    f32x16 s;
+    if (j0 - p_hi >= a.md || j0 + 31 - p_lo <= -a.md) {
+      s = splat16(j0 > p_lo ? right : left);
+    } else {  // a few tiles of a long context: gathered from the cached table
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        s[r] = bias_entry(a, min(max(j0 + 8 * (r >> 2) + 4 * hi + (r & 3) - p, -a.md), a.md), hc);
+    }
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks) s = E::mma(kf[ks], qf[ks], s);
+#pragma unroll
+    for (int n = 0; n < NV; ++n) *reinterpret_cast<u32x4*>(sV + tile_at<DP>(n * RPI + lane / CPR, lane % CPR)) = vr[n];
+    if (t + 4 < t1) load(t + 4);
+    if (j0 + 32 > sq.klen || (a.causal && j0 + 31 > p_lo)) {
+      const int lim = (a.causal ? min(sq.klen, p + 1) : sq.klen) - j0 - 4 * hi;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r >> 2) + (r & 3) >= lim) s[r] = -RB_INF;
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    mx = half_max(mx);
+    if (__any((mx - m) * a.c2 > 8.f)) {  // as in rb_fwd_kernel
+      const float up = fmaxf(m, mx);
+      const float al = up == -RB_INF ? 1.f : __builtin_amdgcn_exp2f((m - up) * a.c2);
+      m = up;
+      l *= al;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= al;
+    }
+    const float mc = m == -RB_INF ? 0.f : m * a.c2;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, -mc));
+      l += s[r];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's V tile is written before other lanes read it
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      const u32x4 pb = pack8<E>(s, 8 * kk);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] = E::mma(frag_t<DP>(sV, 16 * kk, d, lane), pb, o[d]);
+    }
+    __builtin_amdgcn_wave_barrier();
   }
-  d = sum8(d);
-  d += dpp_mov<DPP_MIRROR>(d);
-  if (c == 0) {
-    const int64_t at = ((int64_t)b * a.H + h) * a.Tq + i;
-    const float s = i < sq.qlen ? a.lse_in[at] : -RB_INF;
-    a.delta[at] = d;
-    a.lse2[at] = s == -RB_INF ? RB_INF : s * RB_LOG2E;
+
+  // join the 4 waves: reference, sum, rows of O [32][DP + 4] f32 (the padding spreads a column's 32 rows over the banks)
+  l = half_sum(l);
+  float* const sO = reinterpret_cast<float*>(smem);
+  float* const sM = sO + 32 * (DP + 4);  // [4][2][32]
+  __syncthreads();                       // the V tiles are read
+  if (hi == 0) sM[wave * 64 + n32] = m, sM[wave * 64 + 32 + n32] = l;
+  __syncthreads();
+  float mall = sM[n32], lall = 0.f;
+#pragma unroll
+  for (int w = 1; w < 4; ++w) mall = fmaxf(mall, sM[w * 64 + n32]);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float mw = sM[w * 64 + n32];
+    lall += mw == -RB_INF ? 0.f : sM[w * 64 + 32 + n32] * __builtin_amdgcn_exp2f((mw - mall) * a.c2);
   }
+  const float mine = m == -RB_INF ? 0.f : __builtin_amdgcn_exp2f((m - mall) * a.c2);
+  for (int w = 0; w < 4; ++w) {  // in order
+    if (wave == w) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          f32x4* const at = reinterpret_cast<f32x4*>(sO + n32 * (DP + 4) + 32 * d + 8 * g + 4 * hi);
+          f32x4 x = {o[d][4 * g] * mine, o[d][4 * g + 1] * mine, o[d][4 * g + 2] * mine, o[d][4 * g + 3] * mine};
+          if (m == -RB_INF) x = f32x4{0.f, 0.f, 0.f, 0.f};
+          *at = w == 0 ? x : *at + x;
+        }
+    }
+    __syncthreads();
+  }
+  if (wave == 0 && hi == 0) sM[n32] = mall, sM[32 + n32] = valid ? lall : 0.f;
+  __syncthreads();
+  const int rows = min(32, R - rb * 32);
+  if (a.nsplit == 1) {
+    for (int x = tid; x < rows * (DP / 4); x += 256) {
+      const int r = x / (DP / 4), c = x % (DP / 4) * 4, rr = rb * 32 + r;
+      if (c >= a.D) continue;
+      const float sum = sM[32 + r], inv = 1.f / sum;
+      const f32x4 y = *reinterpret_cast<const f32x4*>(sO + r * (DP + 4) + c);
+      uint16_t* const op = a.out + b * a.so.b + (int64_t)(rr / G) * a.so.t + (hk * G + rr % G) * a.so.h + c;
+      if (sum == 0.f) store4<E>(op, 0.f, 0.f, 0.f, 0.f);
+      else store4<E>(op, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+    }
+    if (a.lse != nullptr && tid < rows) {
+      const int rr = rb * 32 + tid;
+      const float sum = sM[32 + tid];
+      a.lse[((int64_t)b * a.H + hk * G + rr % G) * a.Tq + rr / G] =
+          sum == 0.f ? -RB_INF : (sM[tid] * a.c2 + __builtin_amdgcn_logf(sum)) * RB_LN2;
+    }
+    return;
+  }
+  // workspace: O rows [row][split][DP], then (reference, sum) [row][split]
+  const int64_t first = (int64_t)bk * R + rb * 32;
+  for (int x = tid; x < rows * (DP / 4); x += 256) {
+    const int r = x / (DP / 4), c = x % (DP / 4) * 4;
+    *reinterpret_cast<f32x4*>(a.part + ((first + r) * a.nsplit + split) * DP + c) = *reinterpret_cast<const f32x4*>(sO + r * (DP + 4) + c);
+  }
+  float2* const ml = reinterpret_cast<float2*>(a.part + (int64_t)a.B * a.Hk * R * a.nsplit * DP);
+  if (tid < rows) ml[(first + tid) * a.nsplit + split] = make_float2(sM[tid] * a.c2, sM[32 + tid]);
+}
+
+// one wave per row: the splits' states in order, 64 at a time (their weights in the lanes, so that the loads of O do not wait)
+template <class E, int DP>
+__global__ __launch_bounds__(256) void rb_join_kernel(RbArgs a) {
+  const int G = a.H / a.Hk, R = a.Tq * G, lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), nrow = (int64_t)a.B * a.Hk * R;
+  if (row >= nrow) return;
+  const float2* const ml = reinterpret_cast<const float2*>(a.part + nrow * a.nsplit * DP) + row * a.nsplit;
+  constexpr int N = DP == 128 ? 2 : 1;
+  float m = -RB_INF, sum = 0.f, o[N] = {};
+  for (int s0 = 0; s0 < a.nsplit; s0 += 64) {
+    const int n = min(64, a.nsplit - s0);
+    float2 x = make_float2(-RB_INF, 0.f);
+    if (lane < n) x = ml[s0 + lane];
+    if (x.y == 0.f) x.x = -RB_INF;
+    const float up = fmaxf(m, wave_max(x.x));
+    if (up == -RB_INF) continue;
+    const float al = __builtin_amdgcn_exp2f(m - up), w = x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - up);
+    m = up;
+    sum = sum * al + wave_sum(x.y * w);
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] *= al;
+    const float* const op = a.part + (row * a.nsplit + s0) * DP + (DP == 128 ? 2 : 1) * (lane & (DP - 1));
+    for (int s = 0; s < n; s += 8)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {  // (behind the last split: its row again, with weight 0)
+        const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s + e));
+        const float* const at = op + min(s + e, n - 1) * DP;
+        if constexpr (DP == 128) {
+          const float2 y = *reinterpret_cast<const float2*>(at);
+          o[0] += y.x * ws;
+          o[1] += y.y * ws;
+        } else {
+          o[0] += *at * ws;
+        }
+      }
+  }
+  const int64_t bk = row / R;
+  const int rr = (int)(row % R), b = (int)(bk / a.Hk), h = (int)(bk % a.Hk) * G + rr % G, i = rr / G;
+  uint16_t* const at = a.out + b * a.so.b + (int64_t)i * a.so.t + h * a.so.h;
+  const float inv = 1.f / sum;
+  if constexpr (DP == 128) {
+    if (2 * lane < a.D) *reinterpret_cast<unsigned*>(at + 2 * lane) = sum == 0.f ? 0u : E::pack(o[0] * inv, o[1] * inv);
+  } else {
+    if (lane < a.D) at[lane] = sum == 0.f ? (uint16_t)0 : (uint16_t)E::pack(o[0] * inv, 0.f);
+  }
+  if (a.lse != nullptr && lane == 0) a.lse[((int64_t)b * a.H + h) * a.Tq + i] = sum == 0.f ? -RB_INF : (m + __builtin_amdgcn_logf(sum)) * RB_LN2;
+}
+
+// =============================================================================================== backward
+// The table's gradient is the sum of dS along diagonals (equal distance r).  A lane holds one query and groups of four
+// consecutive keys, and a diagonal runs through neighbouring lanes, so a group is summed along its diagonals by three DPP
+// additions that pass the partial sums one lane up:  N = x3 + up(x2 + up(x1 + up(x0))): lane i then holds the sum of distance
+// r = k0 + 3 - i.  What passes from lane 31 to lane 32 (from 63 to 0) belongs to the same distance as lanes 0..2 of the SAME half
+// 32 keys before: lanes 0..2 of a half separate their own part (`own`, a chain that starts at their half) from what came
+// over, which is added to the part kept from 32 keys before, `kept`.  So each (group, half) writes 32 neighbouring cells of its own
+// array per sub-tile, cells that the other waves do not touch in the same step (their queries are 32 further): plain
+// read-add-write with a barrier per step, no atomics, and a fixed order.  11 vector instructions per group of four; ds_add_f32
+// took 187 cycles per instruction here (124 us for the 32 x 400 backward's dq kernel).
+constexpr int DPP_WAVE_ROR1 = 0x13c, DPP_ROW_SHR1 = 0x111;
+DEV float from_below(float x) { return dpp_mov<DPP_WAVE_ROR1>(x); }      // lane l: the value of lane l - 1, lane 0: of lane 63
+DEV float from_below_row(float x) { return dpp_mov<DPP_ROW_SHR1>(x); }   // within 16 lanes, 0 enters
+DEV float swap_halves(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const unsigned a0 = r[0], a1 = r[1];
+  return __uint_as_float((threadIdx.x & 32) ? a0 : a1);
 }
 
 // dq and the table's gradient: 4 waves x 32 queries of one (sequence, head) against 64-key tiles.
 //   S^T = K Q^T (+ bias), dP^T = V dO^T (from -delta), dS = P dP, dQ^T += K^T dS^T
-// The table's gradient is the sum of dS along diagonals.  Far tiles add to one number per lane and side; in near tiles every
-// dS goes to its distance's cell in LDS by ds_add_f32, into a copy per half wave: lanes of one half hold 32 different
-// distances, and the LDS instructions of a wave run in order, so the result does not depend on timing.
+// It also leaves delta_i = do_i . o_i and the rows' log-sum-exp in log2 units for the next kernel, +inf where a row has no
+// keys or lies behind its sequence (exp2(s - inf) = 0: such rows drop out of every product).
 template <class E, int DP>
-__global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
+__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dq_kernel(RbArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   constexpr int P = 2 * DP, TILE = 64 * P, NK = DP / 16, ND = DP / 32;
   unsigned char* const sK = smem;
   unsigned char* const sV = smem + 2 * TILE;
   float* const sB = reinterpret_cast<float*>(smem + 4 * TILE);
   const int span = 2 * (a.md + RB_PAD) + 1;
-  float* const sG = sB + span;  // [8][span]
-  float* const sFar = sG + 8 * span;  // [4][2]
+  float* const sG = sB + span;                                      // [4 groups][2 halves][span]
+  double* const sFar = reinterpret_cast<double*>(smem + 4 * TILE + ((9 * span + 1) / 2 * 2) * 4);  // [4][2]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, n32 = lane & 31;
   const int id = xcd_order(blockIdx.x, a.nblk);
   const int bh = id / a.ntile, tile = a.ntile - 1 - id % a.ntile;
@@ -406,12 +613,26 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   u32x4 qf[NK], df[NK];
   row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, i, i < sq.qlen, a.D, hi, qf);
   row_frags<DP>(a.dout + b * a.sdo.b + h * a.sdo.h, a.sdo.t, i, i < sq.qlen, a.D, hi, df);
-  const int64_t at = ((int64_t)b * a.H + h) * a.Tq + i;
-  const float lse2 = i < a.Tq ? a.lse2[at] : RB_INF, delta = i < a.Tq ? a.delta[at] : 0.f;
+  float delta = 0.f, lse2 = RB_INF;
+  {
+    u32x4 of[NK];
+    row_frags<DP>(a.o + b * a.so.b + h * a.so.h, a.so.t, i, i < sq.qlen, a.D, hi, of);
+    const int64_t at = ((int64_t)b * a.H + h) * a.Tq + i;
+    const float x = i < sq.qlen ? a.lse_in[at] : -RB_INF;
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) delta += E::lo(df[ks][e]) * E::lo(of[ks][e]) + E::hi(df[ks][e]) * E::hi(of[ks][e]);
+    delta = half_sum(delta);
+    if (x != -RB_INF) lse2 = x * RB_LOG2E;
+    if (hi == 0 && i < a.Tq) a.delta[at] = delta, a.lse2[at] = lse2;
+  }
   f32x16 dq[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dq[d] = splat16(0.f);
-  float farl = 0.f, farr = 0.f;
+  double farl = 0., farr = 0.;   // 64 bits: thousands of terms of both signs
+  float kept[4] = {0.f, 0.f, 0.f, 0.f};
+  bool pending = false;
   spread_table(a, h, sB, tid, 256);
   for (int x = tid; x < 8 * span; x += 256) sG[x] = 0.f;
   if (nt > 0) {
@@ -420,7 +641,8 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   }
   __syncthreads();
   const float left = sB[0], right = sB[span - 1];
-  float* const gp0 = sG + (wave * 2 + hi) * span + (4 * hi - p0 - n32 + a.md + RB_PAD);
+  // lane's cell for key base 0: its own class (half), or for lanes 0..2 the other half's, 32 keys before
+  const int cls = n32 < 3 ? hi ^ 1 : hi, cell0 = cls * span + 4 * cls + 3 - n32 - (n32 < 3 ? 32 : 0) - p0 + a.md + RB_PAD;
 
   for (int t = 0; t < nt; ++t) {
     const int j0 = t * 64;
@@ -431,50 +653,70 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
     }
     const unsigned char* const kt = sK + (t & 1) * TILE;
     const unsigned char* const vt = sV + (t & 1) * TILE;
-    if (j0 < wend) {
-      const bool far = j0 - (p0 + 31) >= a.md || j0 + 63 - p0 <= -a.md;
-      const bool edge = j0 + 64 > sq.klen || (a.causal && j0 + 63 > p0);
-      const int lim = (a.causal ? min(sq.klen, p0 + n32 + 1) : sq.klen) - j0 - 4 * hi;
+    const bool active = j0 < wend;
+    const bool near = active && j0 - (p0 + 31) < a.md && j0 + 63 - p0 > -a.md;
+    const int pw = sq.off + q0;
+    const bool any_near = j0 - (pw + 127) < a.md && j0 + 63 - pw > -a.md;  // of any wave: they share the barrier
+    if (!near && pending) {  // the last parts kept have nothing to wait for
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        f32x16 s, dp = splat16(-delta);
-        if (far) {
-          s = splat16(j0 > p0 ? right : left);
-        } else {
-          const float* const bp = sB + (j0 - p0 - n32 + 4 * hi + 32 * u + a.md + RB_PAD);
+      for (int g = 0; g < 4; ++g)
+        if (n32 < 3) sG[2 * g * span + cell0 + j0 + 8 * g] += kept[g];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = bp[8 * (r >> 2) + (r & 3)];
+      for (int g = 0; g < 4; ++g) kept[g] = 0.f;
+      pending = false;
+    }
+    const bool edge = j0 + 64 > sq.klen || (a.causal && j0 + 63 > p0);
+    const int lim = (a.causal ? min(sq.klen, p0 + n32 + 1) : sq.klen) - j0 - 4 * hi;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (u == 1 && any_near) __syncthreads();
+      if (!active) continue;
+      f32x16 s, dp = splat16(-delta);
+      if (near) {
+        const float* const bp = sB + (j0 - p0 - n32 + 4 * hi + 32 * u + a.md + RB_PAD);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = bp[8 * (r >> 2) + (r & 3)];
+      } else {
+        s = splat16(j0 > p0 ? right : left);
+      }
+#pragma unroll
+      for (int ks = 0; ks < NK; ++ks) {
+        s = E::mma(frag<DP>(kt, 32 * u + n32, ks, hi), qf[ks], s);
+        dp = E::mma(frag<DP>(vt, 32 * u + n32, ks, hi), df[ks], dp);
+      }
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * u + 8 * (r >> 2) + (r & 3) >= lim) s[r] = -RB_INF;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, -lse2)) * dp[r];
+      if (near) {
+        float old[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) old[g] = sG[2 * g * span + cell0 + j0 + 32 * u + 8 * g];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float all = s[4 * g + 3] + from_below(s[4 * g + 2] + from_below(s[4 * g + 1] + from_below(s[4 * g])));
+          const float own = s[4 * g + 3] + from_below_row(s[4 * g + 2] + from_below_row(s[4 * g + 1]));
+          const float x = n32 < 3 ? (all - own) + kept[g] : all;
+          kept[g] = swap_halves(own);
+          sG[2 * g * span + cell0 + j0 + 32 * u + 8 * g] = old[g] + x;
         }
+        pending = true;
+      } else {
+        float x[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int ks = 0; ks < NK; ++ks) {
-          s = E::mma(frag<DP>(kt, 32 * u + n32, ks, hi), qf[ks], s);
-          dp = E::mma(frag<DP>(vt, 32 * u + n32, ks, hi), df[ks], dp);
-        }
-        if (edge) {
+        for (int r = 4; r < 16; ++r) x[r & 3] += s[r];
+        const double y = (double)((x[0] + x[1]) + (x[2] + x[3]));
+        if (j0 > p0) farr += y;
+        else farl += y;
+      }
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (32 * u + 8 * (r >> 2) + (r & 3) >= lim) s[r] = -RB_INF;
-        }
+      for (int kk = 0; kk < 2; ++kk) {
+        const u32x4 ds = pack8<E>(s, 8 * kk);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, -lse2)) * dp[r];
-        if (far) {
-          float x = 0.f;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) x += s[r];
-          if (j0 > p0) farr += x;
-          else farl += x;
-        } else {
-          float* const gp = gp0 + j0 + 32 * u;
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            __hip_atomic_fetch_add(gp + 8 * (r >> 2) + (r & 3), s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-        }
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          const u32x4 ds = pack8<E>(s, 8 * kk);
-#pragma unroll
-          for (int d = 0; d < ND; ++d) dq[d] = E::mma(frag_t<DP>(kt, 32 * u + 16 * kk, d, lane), ds, dq[d]);
-        }
+        for (int d = 0; d < ND; ++d) dq[d] = E::mma(frag_t<DP>(kt, 32 * u + 16 * kk, d, lane), ds, dq[d]);
       }
     }
     if (more) {
@@ -482,6 +724,11 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
       lv.store(sV + ((t + 1) & 1) * TILE, tid, lv.r);
     }
     __syncthreads();
+  }
+  if (pending) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      if (n32 < 3) sG[2 * g * span + cell0 + nt * 64 + 8 * g] += kept[g];
   }
 
   if (i < a.Tq) {
@@ -495,9 +742,12 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
           store4<E>(op + c, dq[d][4 * g] * a.scale, dq[d][4 * g + 1] * a.scale, dq[d][4 * g + 2] * a.scale, dq[d][4 * g + 3] * a.scale);
       }
   }
-  // the workgroup's share of the table's gradient, by distance: copies in order, then what lies beyond the largest distance
-  farl = wave_sum(farl);
-  farr = wave_sum(farr);
+  // the workgroup's share of the table's gradient: by distance (arrays in order), then by bucket
+#pragma unroll
+  for (int w = 1; w < 64; w <<= 1) {
+    farl += __shfl_xor(farl, w);
+    farr += __shfl_xor(farr, w);
+  }
   if (lane == 0) sFar[2 * wave] = farl, sFar[2 * wave + 1] = farr;
   __syncthreads();
   for (int x = tid; x < span; x += 256) {
@@ -507,44 +757,43 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
     sB[x] = y;
   }
   __syncthreads();
-  float* const part = a.part + (int64_t)id * (2 * a.md + 1);
-  for (int x = 1 + tid; x < 2 * a.md; x += 256) part[x] = sB[x + RB_PAD];
-  if (wave < 2) {  // the two ends: entries 0 .. PAD and the last PAD + 1
-    float y = 0.f;
-    for (int x = lane; x <= RB_PAD; x += 64) y += sB[wave == 0 ? x : span - 1 - x];
-    y = wave_sum(y);
-    if (lane == 0) part[wave == 0 ? 0 : 2 * a.md] = y + ((sFar[wave] + sFar[2 + wave]) + (sFar[4 + wave] + sFar[6 + wave]));
+  if (wave < 2) {  // the two ends hold everything beyond them
+    double y = 0.;
+    for (int x = lane; x <= RB_PAD; x += 64) y += (double)sB[wave == 0 ? x : span - 1 - x];
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) y += __shfl_xor(y, w);
+    if (lane == 0) sFar[wave] = y + ((sFar[wave] + sFar[2 + wave]) + (sFar[4 + wave] + sFar[6 + wave]));
+  }
+  __syncthreads();
+  const int nwg = a.B * a.ntile, wg = b * a.ntile + tile;
+  for (int n = tid; n < a.nb; n += 256) {
+    const int lo = a.bucket_range[2 * n], end = a.bucket_range[2 * n + 1];
+    double y = 0.;
+    for (int r = lo; r < end; ++r) y += r == -a.md ? sFar[0] : r == a.md ? sFar[1] : (double)sB[r + a.md + RB_PAD];
+    a.part[((int64_t)h * a.nb + n) * nwg + wg] = (float)y;
   }
 }
 
-// dtable[n, h] = sum over the workgroups of head h and the distances of bucket n, in 64 bits and a fixed order
-__global__ __launch_bounds__(256) void rb_table_kernel(RbArgs a) {
-  __shared__ double red[256];
-  const int n = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-  const int lo = a.bucket_range[2 * n], width = a.bucket_range[2 * n + 1] - lo;  // distances lo .. lo + width - 1
-  const int64_t total = (int64_t)a.B * a.ntile * width;
+// dtable[n, h] = sum over the workgroups of head h, in 64 bits and a fixed order; one wave per entry
+DEV void table_sum(const RbArgs& a, int entry, int nwg) {
+  if (entry >= a.nb * a.H) return;
+  const int lane = threadIdx.x & 63, h = entry / a.nb, n = entry % a.nb;
   double s = 0.;
-  for (int64_t x = tid; x < total; x += 256) {
-    const int64_t wg = x / width;
-    const int r = (int)(x % width);
-    const int64_t id = ((wg / a.ntile) * a.H + h) * a.ntile + wg % a.ntile;
-    s += (double)a.part[id * (2 * a.md + 1) + lo + a.md + r];
-  }
-  red[tid] = s;
-  __syncthreads();
+  for (int x = lane; x < nwg; x += 64) s += (double)a.part[(int64_t)entry * nwg + x];
 #pragma unroll
-  for (int w = 128; w > 0; w >>= 1) {
-    if (tid < w) red[tid] += red[tid + w];
-    __syncthreads();
-  }
-  if (tid == 0) a.dtable[(int64_t)n * a.H + h] = (float)red[0];
+  for (int w = 1; w < 64; w <<= 1) s += __shfl_xor(s, w);
+  if (lane == 0) a.dtable[n * a.H + h] = (float)s;
 }
 
 // dk and dv: 4 waves x 32 keys of one (sequence, key head) against 64-query tiles of every head of its group.
 //   S = Q K^T (+ bias), dP = dO V^T (from -delta), dV^T += dO^T P, dK^T += Q^T dS
 template <class E, int DP>
-__global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
+__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  if ((int)blockIdx.x >= a.nblk) {  // the last workgroups: the table's gradient from the dq kernel's shares
+    table_sum(a, (blockIdx.x - a.nblk) * 4 + (threadIdx.x >> 6), a.B * a.nqtile);
+    return;
+  }
   constexpr int P = 2 * DP, TILE = 64 * P, NK = DP / 16, ND = DP / 32;
   unsigned char* const sQ = smem;
   unsigned char* const sO = smem + 2 * TILE;
@@ -705,7 +954,7 @@ RbArgs to_args(const csship_relbias* p) {
 }
 
 size_t fwd_lds(int DP, int md) { return (size_t)4 * 64 * 2 * DP + (2 * (md + RB_PAD) + 1) * 4; }
-size_t dq_lds(int DP, int md) { return (size_t)4 * 64 * 2 * DP + (size_t)9 * (2 * (md + RB_PAD) + 1) * 4 + 32; }
+size_t dq_lds(int DP, int md) { return (size_t)4 * 64 * 2 * DP + (size_t)(9 * (2 * (md + RB_PAD) + 1) + 1) / 2 * 2 * 4 + 64; }
 size_t dkv_lds(int DP, int md) { return fwd_lds(DP, md) + 1024; }
 
 // launches with more than 64 KB of LDS have to be allowed, per device: asked for at each such launch
@@ -719,8 +968,32 @@ int launch(K kernel, int64_t blocks, size_t lds, const RbArgs& a, hipStream_t s)
   return CSSHIP_OK;
 }
 
+// Which forward: rb_fwd_kernel reuses a K / V tile for 128 queries, rb_few_kernel for 32 rows but may take all heads of a group at
+// once and split the keys.  The latter where the former would leave most of the chip idle.
+struct FwdPlan { bool few; int ntile, nsplit; };
+FwdPlan fwd_plan(const csship_relbias* p) {
+  const int64_t rows = (int64_t)p->Tq * (p->H / p->Hk), tiles = (rows + 31) / 32, wide = (int64_t)p->B * p->H * ((p->Tq + 127) / 128);
+  FwdPlan f{rows <= 32 || (wide < 128 && p->Tk >= 1024), (int)tiles, 1};
+  if (f.few && p->Tk > 1024) {  // 1024 keys and less: 8 tiles a wave, no second launch
+    const int64_t want = 768 / ((int64_t)p->B * p->Hk * tiles), most = (p->Tk + 511) / 512;
+    f.nsplit = (int)(want < 1 ? 1 : want < most ? want : most);
+  }
+  return f;
+}
+int width_of(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+
 template <class E, int DP>
-int launch_fwd(RbArgs a, hipStream_t s) {
+int launch_fwd(RbArgs a, const csship_relbias* p, hipStream_t s) {
+  const FwdPlan f = fwd_plan(p);
+  if (f.few) {
+    a.ntile = f.ntile;
+    a.nsplit = f.nsplit;
+    a.nblk = a.B * a.Hk * a.ntile * a.nsplit;
+    const size_t tiles = 4 * 32 * 2 * DP, join = (32 * (DP + 4) + 256) * 4;
+    if (const int rc = launch(rb_few_kernel<E, DP>, a.nblk, tiles > join ? tiles : join, a, s)) return rc;
+    if (a.nsplit == 1) return CSSHIP_OK;
+    return launch(rb_join_kernel<E, DP>, ((int64_t)a.B * a.H * a.Tq + 3) / 4, 0, a, s);
+  }
   a.ntile = (a.Tq + 127) / 128;
   a.nblk = a.B * a.H * a.ntile;
   if (a.nblk == 0) return CSSHIP_OK;
@@ -729,29 +1002,22 @@ int launch_fwd(RbArgs a, hipStream_t s) {
 
 template <class E, int DP>
 int launch_bwd(RbArgs a, hipStream_t s) {
-  const int64_t rows = (int64_t)a.B * a.Tq * a.H;
-  if (rows > 0)
-    if (const int rc = launch(rb_rows_kernel<E>, (rows + 15) / 16, 0, a, s)) return rc;
-  RbArgs d = a;
-  d.ntile = (a.Tq + 127) / 128;
-  d.nblk = a.B * a.H * d.ntile;
-  if (d.nblk > 0)
-    if (const int rc = launch(rb_dq_kernel<E, DP>, d.nblk, dq_lds(DP, a.md), d, s)) return rc;
-  RbArgs e = a;
-  e.ntile = (a.Tk + 127) / 128;
-  e.nblk = a.B * a.Hk * e.ntile;
-  if (e.nblk > 0)
-    if (const int rc = launch(rb_dkv_kernel<E, DP>, e.nblk, dkv_lds(DP, a.md), e, s)) return rc;
-  rb_table_kernel<<<dim3(a.nb, a.H), 256, 0, s>>>(d);
-  CSSHIP_CHECK_LAUNCH();
-  return CSSHIP_OK;
+  a.ntile = a.nqtile = (a.Tq + 127) / 128;
+  a.nblk = a.B * a.H * a.ntile;
+  if (a.nblk > 0)
+    if (const int rc = launch(rb_dq_kernel<E, DP>, a.nblk, dq_lds(DP, a.md), a, s)) return rc;
+  a.ntile = (a.Tk + 127) / 128;
+  a.nblk = a.B * a.Hk * a.ntile;
+  return launch(rb_dkv_kernel<E, DP>, (int64_t)a.nblk + (a.nb * a.H + 3) / 4, dkv_lds(DP, a.md), a, s);
 }
 
 template <class E>
-int by_width(const RbArgs& a, bool bwd, hipStream_t s) {
-  if (a.D <= 32) return bwd ? launch_bwd<E, 32>(a, s) : launch_fwd<E, 32>(a, s);
-  if (a.D <= 64) return bwd ? launch_bwd<E, 64>(a, s) : launch_fwd<E, 64>(a, s);
-  return bwd ? launch_bwd<E, 128>(a, s) : launch_fwd<E, 128>(a, s);
+int fwd_by_width(const RbArgs& a, const csship_relbias* p, hipStream_t s) {
+  return a.D <= 32 ? launch_fwd<E, 32>(a, p, s) : a.D <= 64 ? launch_fwd<E, 64>(a, p, s) : launch_fwd<E, 128>(a, p, s);
+}
+template <class E>
+int bwd_by_width(const RbArgs& a, hipStream_t s) {
+  return a.D <= 32 ? launch_bwd<E, 32>(a, s) : a.D <= 64 ? launch_bwd<E, 64>(a, s) : launch_bwd<E, 128>(a, s);
 }
 
 int64_t row_words(const csship_relbias* p) { return ((int64_t)p->B * p->H * p->Tq + 3) / 4 * 4; }
@@ -761,15 +1027,18 @@ int64_t row_words(const csship_relbias* p) { return ((int64_t)p->B * p->H * p->T
 extern "C" {
 
 size_t csship_relbias_fwd_workspace(const csship_relbias* p) {
-  (void)p;
-  return 0;
+  if (check_args(p) != CSSHIP_OK || p->B == 0 || p->Tq == 0) return 0;
+  const FwdPlan f = fwd_plan(p);
+  return f.nsplit == 1 ? 0 : (size_t)p->B * p->H * p->Tq * f.nsplit * (width_of(p->D) + 2) * 4;
 }
 
 int csship_relbias_fwd(const csship_relbias* p, uint16_t* out, const int64_t* out_stride, float* lse, void* workspace,
                        size_t workspace_bytes, csship_stream_t stream) {
   if (const int rc = check_args(p)) return rc;
-  (void)workspace;
-  if (workspace_bytes < csship_relbias_fwd_workspace(p)) return CSSHIP_EWORKSPACE;
+  const size_t need = csship_relbias_fwd_workspace(p);
+  if (need > 0 && workspace == nullptr) return CSSHIP_ENULL;
+  if (workspace_bytes < need) return CSSHIP_EWORKSPACE;
+  if (!aligned16(workspace)) return CSSHIP_EALIGN;
   if (p->B == 0 || p->Tq == 0) return CSSHIP_OK;
   if (out == nullptr || out_stride == nullptr) return CSSHIP_ENULL;
   if (!aligned8(out) || !strides_ok(out_stride)) return CSSHIP_EALIGN;
@@ -777,13 +1046,14 @@ int csship_relbias_fwd(const csship_relbias* p, uint16_t* out, const int64_t* ou
   a.out = out;
   a.so = to_strides(out_stride);
   a.lse = lse;
-  return p->dtype == CSSHIP_RELBIAS_BF16 ? by_width<ElemBf>(a, false, as_stream(stream)) : by_width<ElemHf>(a, false, as_stream(stream));
+  a.part = static_cast<float*>(workspace);
+  return p->dtype == CSSHIP_RELBIAS_BF16 ? fwd_by_width<ElemBf>(a, p, as_stream(stream)) : fwd_by_width<ElemHf>(a, p, as_stream(stream));
 }
 
 size_t csship_relbias_bwd_workspace(const csship_relbias* p) {
   if (check_args(p) != CSSHIP_OK) return 0;
   const int64_t wgs = (int64_t)p->B * p->H * ((p->Tq + 127) / 128);
-  return (size_t)(2 * row_words(p) + wgs * (2 * p->max_distance + 1)) * 4 + 16;
+  return (size_t)(2 * row_words(p) + wgs * p->n_buckets) * 4 + 16;
 }
 
 int csship_relbias_bwd(const csship_relbias* p, const uint16_t* out, const int64_t* out_stride, const float* lse, const uint16_t* dout,
@@ -812,7 +1082,7 @@ int csship_relbias_bwd(const csship_relbias* p, const uint16_t* out, const int64
   a.delta = static_cast<float*>(workspace);
   a.lse2 = a.delta + row_words(p);
   a.part = a.lse2 + row_words(p);
-  return p->dtype == CSSHIP_RELBIAS_BF16 ? by_width<ElemBf>(a, true, as_stream(stream)) : by_width<ElemHf>(a, true, as_stream(stream));
+  return p->dtype == CSSHIP_RELBIAS_BF16 ? bwd_by_width<ElemBf>(a, as_stream(stream)) : bwd_by_width<ElemHf>(a, as_stream(stream));
 }
 
 }  // extern "C"

@@ -324,25 +324,37 @@ def _relbias_rows(t, name, like=None):
     """A [B, T, heads, D] operand whose rows csship_relbias can address (a copy where its strides do not allow it)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f"css_amd: '{name}' must be a CUDA/HIP tensor (no CPU path exists)")
-    if t.dim() != 4:
+    s, dt = t.stride(), t.dtype
+    if len(s) != 4:
         raise RuntimeError(f"css_amd: '{name}' must be [batch, frames, heads, width], got {tuple(t.shape)}")
-    if t.dtype not in (torch.bfloat16, torch.float16) or (like is not None and t.dtype != like.dtype):
-        raise TypeError(f"css_amd: '{name}' must be {'bfloat16 or float16' if like is None else like.dtype}, got {t.dtype}")
-    if like is not None and t.device != like.device:
-        raise RuntimeError(f"css_amd: '{name}' is on {t.device}, the queries on {like.device}")
-    s = t.stride()
+    if like is None:
+        if dt is not torch.bfloat16 and dt is not torch.float16:
+            raise TypeError(f"css_amd: '{name}' must be bfloat16 or float16, got {dt}")
+    else:
+        if dt is not like.dtype:
+            raise TypeError(f"css_amd: '{name}' must be {like.dtype}, got {dt}")
+        if t.get_device() != like.get_device():
+            raise RuntimeError(f"css_amd: '{name}' is on {t.device}, the queries on {like.device}")
     if s[3] != 1 or (s[0] | s[1] | s[2]) & 7 or s[1] >= 1 << 23 or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _relbias_struct(q, k, v, table, buckets, scale, causal, offset, k_lens, q_lens):
-    """Checks the operands of csship_relbias and fills its struct; returns (struct, tensors it points to)."""
+def _relbias_words(x, name, B, like):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"css_amd: '{name}' must be an int32 tensor or None")
+    if x.dtype is not torch.int32 or tuple(x.shape) != (B,) or x.get_device() != like.get_device() or not x.is_contiguous():
+        raise RuntimeError(f"css_amd: '{name}' must be a dense int32 [{B}] on {like.device}")
+    return x.data_ptr()
+
+
+def _relbias_pack(q, k, v, table, buckets, scale, causal, offset, k_lens, q_lens):
+    """Checks the operands of csship_relbias; returns (its bytes, q, k, v, table), the tensors as they are pointed to."""
     q = _relbias_rows(q, "q")
     k, v = _relbias_rows(k, "k", q), _relbias_rows(v, "v", q)
     B, Tq, H, D = q.shape
-    Tk, Hk = k.shape[1], k.shape[2]
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+    Bk, Tk, Hk, Dk = k.shape
+    if Bk != B or Dk != D or v.shape != k.shape:
         raise RuntimeError(f"css_amd: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not belong together")
     if Hk < 1 or H < 1 or H % Hk:
         raise RuntimeError(f"css_amd: {H} query heads cannot share {Hk} key heads evenly")
@@ -350,33 +362,30 @@ def _relbias_struct(q, k, v, table, buckets, scale, causal, offset, k_lens, q_le
         raise RuntimeError(f"css_amd: head width {D}: a multiple of 8 up to 128")
     _need(table, torch.float32, "table")
     n, far = int(buckets[0]), int(buckets[1])
-    if tuple(table.shape) != (n, H) or table.device != q.device:
+    if tuple(table.shape) != (n, H) or table.get_device() != q.get_device():
         raise RuntimeError(f"css_amd: 'table' must be [{n}, {H}] on {q.device}, got {tuple(table.shape)} on {table.device}")
-    table = table.detach().contiguous()
-    for name, x in (("k_lens", k_lens), ("q_lens", q_lens), ("offset", offset)):
-        if isinstance(x, torch.Tensor):
-            if x.dtype != torch.int32 or tuple(x.shape) != (B,) or x.device != q.device or not x.is_contiguous():
-                raise RuntimeError(f"css_amd: '{name}' must be a dense int32 [{B}] on {q.device}")
-        elif x is not None and name != "offset":
-            raise TypeError(f"css_amd: '{name}' must be an int32 tensor or None")
-    each = isinstance(offset, torch.Tensor)
-    if not each and not -(1 << 28) <= int(offset) <= 1 << 28:
+    if not table.is_contiguous():
+        table = table.contiguous()
+    kl = 0 if k_lens is None else _relbias_words(k_lens, "k_lens", B, q)
+    ql = 0 if q_lens is None else _relbias_words(q_lens, "q_lens", B, q)
+    each = 0
+    if isinstance(offset, torch.Tensor):
+        offset, each = 0, _relbias_words(offset, "offset", B, q)
+    elif not -(1 << 28) <= offset <= 1 << 28:
         raise RuntimeError(f"css_amd: offset {offset} out of range")
     scale = D ** -0.5 if scale is None else float(scale)
     if not 1e-6 < scale < 1e6:
         raise RuntimeError(f"css_amd: scale {scale}: a positive number of ordinary size")
     bucket_of, bucket_range = relbias_buckets(buckets, q.device)
-    sq, sk, sv = q.stride(), k.stride(), v.stride()
-    p = _lib.RelBias(q.data_ptr(), k.data_ptr(), v.data_ptr(), sq[:3], sk[:3], sv[:3], table.data_ptr(), bucket_of.data_ptr(),
-                     bucket_range.data_ptr(), k_lens.data_ptr() if k_lens is not None else None,
-                     q_lens.data_ptr() if q_lens is not None else None, offset.data_ptr() if each else None,
-                     _lib.RELBIAS_BF16 if q.dtype == torch.bfloat16 else _lib.RELBIAS_FP16, B, Tq, Tk, H, Hk, D, n, far,
-                     1 if causal else 0, 0 if each else int(offset), scale)
-    return p, (q, k, v, table)
+    p = _lib.RELBIAS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                          table.data_ptr(), bucket_of.data_ptr(), bucket_range.data_ptr(), kl, ql, each,
+                          _lib.RELBIAS_BF16 if q.dtype is torch.bfloat16 else _lib.RELBIAS_FP16, B, Tq, Tk, H, Hk, D, n, far,
+                          1 if causal else 0, int(offset), scale)
+    return p, q, k, v, table
 
 
 def _strides3(t):
-    return _lib._s3(*t.stride()[:3])
+    return _lib.STRIDE3.pack(*t.stride()[:3])
 
 
 def mha_relbias(q, k, v, table, buckets, *, scale=None, causal=False, offset=0, k_lens=None, q_lens=None, want_lse=False):
@@ -388,20 +397,20 @@ def mha_relbias(q, k, v, table, buckets, *, scale=None, causal=False, offset=0, 
     [B] on the device; streaming: frames kept so far); causal: keys behind the query's position are not seen.  k_lens / q_lens
     int32 [B]: lengths of a padded batch; what lies behind them is not read, and those rows of the result are zeros.
     A query without keys gets zeros (log-sum-exp -inf).  -> out [B,Tq,H,D], or (out, lse f32 [B,H,Tq]) with want_lse."""
-    p, keep = _relbias_struct(q, k, v, table, buckets, scale, causal, offset, k_lens, q_lens)
-    q = keep[0]
-    if q.device.index != torch.cuda.current_device():
-        with torch.cuda.device(q.device):
+    p, q, k, v, table = _relbias_pack(q, k, v, table, buckets, scale, causal, offset, k_lens, q_lens)
+    at = q.get_device()
+    if at != torch.cuda.current_device():
+        with torch.cuda.device(at):
             return mha_relbias(q, k, v, table, buckets, scale=scale, causal=causal, offset=offset, k_lens=k_lens, q_lens=q_lens,
                                want_lse=want_lse)
-    B, Tq, H, D = q.shape
-    out = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device)
+    B, Tq, H, _ = q.shape
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((B, H, Tq), dtype=torch.float32, device=q.device) if want_lse else None
     h = lib()
-    n = h.csship_relbias_fwd_workspace(C.byref(p))
+    n = h.csship_relbias_fwd_workspace(p)
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-    check(h.csship_relbias_fwd(C.byref(p), out.data_ptr(), _strides3(out), lse.data_ptr() if want_lse else None,
-                               ws.data_ptr() if n else None, n, torch.cuda.current_stream().cuda_stream))
+    check(h.csship_relbias_fwd(p, out.data_ptr(), _strides3(out), lse.data_ptr() if want_lse else None,
+                               ws.data_ptr() if n else None, n, torch.cuda.current_stream(at).cuda_stream))
     return (out, lse) if want_lse else out
 
 

@@ -805,17 +805,17 @@ def mha_relbias_bwd(q, k, v, table, out, lse, dout, buckets, *, scale=None, caus
     """Backward of ops.mha_relbias (csship_relbias_bwd): (dq, dk, dv, dtable) from the forward's operands, its out and lse
     (want_lse=True) and the gradient of out.  The probabilities are recomputed, nothing of size Tq x Tk is stored; the sums over
     a group's heads, the sequences and the distances of a bucket are taken in a fixed order."""
-    p, keep = ops._relbias_struct(q, k, v, table, buckets, scale, causal, offset, k_lens, q_lens)
-    q, k = keep[0], keep[1]
+    p, q, k, v, table = ops._relbias_pack(q, k, v, table, buckets, scale, causal, offset, k_lens, q_lens)
     B, Tq, H, D = q.shape
     out, dout = ops._relbias_rows(out, "out", q), ops._relbias_rows(dout, "dout", q)
     if out.shape != q.shape or dout.shape != q.shape:
         raise RuntimeError(f"css_amd: out {tuple(out.shape)} and dout {tuple(dout.shape)} must have the shape of q {tuple(q.shape)}")
     _need(lse, torch.float32, "lse")
-    if tuple(lse.shape) != (B, H, Tq) or lse.device != q.device:
+    at = q.get_device()
+    if tuple(lse.shape) != (B, H, Tq) or lse.get_device() != at:
         raise RuntimeError(f"css_amd: 'lse' must be [{B}, {H}, {Tq}] on {q.device}")
-    if q.device.index != torch.cuda.current_device():
-        with torch.cuda.device(q.device):
+    if at != torch.cuda.current_device():
+        with torch.cuda.device(at):
             return mha_relbias_bwd(q, k, v, table, out, lse, dout, buckets, scale=scale, causal=causal, offset=offset,
                                    k_lens=k_lens, q_lens=q_lens)
     lse = lse.contiguous()
@@ -823,12 +823,11 @@ def mha_relbias_bwd(q, k, v, table, out, lse, dout, buckets, *, scale=None, caus
     dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
     dtable = torch.empty(table.shape, dtype=torch.float32, device=q.device)
     h = lib()
-    n = h.csship_relbias_bwd_workspace(C.byref(p))
-    ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
+    ws = torch.empty(h.csship_relbias_bwd_workspace(p), dtype=torch.uint8, device=q.device)
     s3 = ops._strides3
-    check(h.csship_relbias_bwd(C.byref(p), out.data_ptr(), s3(out), lse.data_ptr(), dout.data_ptr(), s3(dout), dq.data_ptr(), s3(dq),
+    check(h.csship_relbias_bwd(p, out.data_ptr(), s3(out), lse.data_ptr(), dout.data_ptr(), s3(dout), dq.data_ptr(), s3(dq),
                                dk.data_ptr(), s3(dk), dv.data_ptr(), s3(dv), dtable.data_ptr(), ws.data_ptr(), ws.numel(),
-                               torch.cuda.current_stream().cuda_stream))
+                               torch.cuda.current_stream(at).cuda_stream))
     return dq, dk, dv, dtable
 
 

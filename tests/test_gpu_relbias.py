@@ -146,6 +146,14 @@ SHAPES = [  # B, Tq, Tk, H, Hk, D, buckets, far, two-sided, causal, offset
     (1, 1, 900, 4, 1, 64, 32, 128, False, True, 899),
     (1, 300, 40, 2, 2, 80, 32, 128, True, True, -100),  # the first 100 queries see no key
     (1, 700, 20, 1, 1, 16, 512, 1024, True, False, 0),
+    # few query rows: one workgroup for all keys, keys split over workgroups, several row blocks, groups of heads in a block
+    (2, 1, 31, 2, 2, 64, 32, 128, True, False, 30),
+    (1, 3, 1500, 8, 2, 128, 32, 128, False, True, 1497),
+    (2, 9, 2100, 12, 4, 64, 320, 800, True, False, 1000),
+    (1, 5, 1100, 14, 2, 32, 16, 40, True, True, 700),
+    (1, 100, 1300, 2, 1, 48, 32, 128, True, False, 1200),
+    (3, 2, 1025, 4, 4, 112, 32, 128, True, True, 0),
+    (1, 1, 2049, 33, 1, 8, 32, 128, True, True, -1),
 ]
 
 
@@ -173,6 +181,18 @@ def test_padded_batch_reads_nothing_behind_its_ends(lib, dtype, causal):
         assert (out[b, n:] == 0).all() and (lse[b, :, n:] == -math.inf).all()
         for name in ("dq", "dk", "dv"):
             assert (got[name][b, n:] == 0).all(), name
+
+
+def test_serving_batch_of_single_frames(lib):
+    """few rows, split keys, lengths and offsets per sequence; an idle slot and garbage behind the kept keys"""
+    lens = [1700, 1, 0, 1024, 33, 1699]
+    q, k, v, table, do = make(8, torch.bfloat16, 6, 1, 1700, 8, 2, 64, 32)
+    for b, n in enumerate(lens):
+        k[b, n:], v[b, n:] = math.nan, math.inf
+    kl = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    for causal in (False, True):
+        out, lse, _ = check_all(lib, q, k, v, table, do, (32, 128), causal=causal, k_lens=kl, offset=(kl - 1).int())
+        assert (out[2] == 0).all() and (lse[2] == -math.inf).all()
 
 
 def test_offsets_per_sequence_and_lengths_outside_the_tensors(lib):
