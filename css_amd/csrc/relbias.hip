@@ -60,10 +60,10 @@ struct RbArgs {
   uint16_t *out, *dq, *dk, *dv;
   float *lse, *dtable;
   const float* lse_in;
-  float *delta, *lse2, *part;  // workspace
+  float *delta, *lse2, *part;  // workspace; delta (negated) and lse2 [B, H, tq128]
   int B, Tq, Tk, H, Hk, D, nb, md, causal, offset;
   float scale, inv_scale, c2;  // c2 = scale * log2(e)
-  int ntile, nblk, nsplit, nqtile;     // row tiles per (sequence, head); workgroups; key ranges (rb_few_kernel)
+  int ntile, nblk, nsplit, nqtile, tq128;     // row tiles per (sequence, head); workgroups; key ranges (rb_few_kernel)
 };
 
 // rows of 2 DP bytes in 16-byte pieces; piece c of row r lies at piece c ^ swz(r).  The key makes both kinds of reads spread over
@@ -116,30 +116,42 @@ DEV float half_sum(float x) {
   return __uint_as_float(a0) + __uint_as_float(a1);
 }
 
-// ---- 64 rows of a [T, heads, D] tensor on their way to LDS: rows and pieces outside (row >= rows, piece >= D / 8) are zeros
-template <int DP, int NT>
-struct Stage {
-  static constexpr int CPR = DP / 8, N = 64 * CPR / NT;
-  u32x4 r[N];
-  DEV void load(const uint16_t* base, int64_t st, int row0, int rows, int D, int tid, u32x4 (&r)[N]) {
-    const __amdgpu_buffer_rsrc_t rs =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base + (int64_t)row0 * st), 0, 0x7ffffff0, 0x00020000);
-    const int left = rows - row0;
+// ---- 64-row tiles of a [T, heads, D] tensor, memory -> LDS without passing registers (buffer_load_dwordx4 ... lds): one
+// instruction of a wave fills 1 KB in lane order, so the swizzle is applied to the address each lane fetches.  Rows at or behind
+// `rows` and pieces at or behind D / 8 lie outside the descriptor: zeros.  Written as inline assembly because the compiler, which
+// cannot tell the double buffer's halves apart, otherwise waits for the transfer before every LDS read behind it; the
+// statement has no result registers, and dma_wait() stands before the barrier that hands the tile over.
+template <int DP>
+struct TileDma {
+  static constexpr int CPR = DP / 8, RPI = 64 / CPR, N = 16 / RPI;  // pieces a row, rows an instruction, instructions a wave
+  unsigned off[N];
+  const uint16_t* base;
+  int64_t st;
+  int rows, D;
+  __device__ __forceinline__ void init(const uint16_t* b, int64_t stride, int rows_, int D_, int wave, int lane) {
+    base = b, st = stride, rows = rows_, D = D_;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int x = tid + n * NT, row = x / CPR, c = x % CPR;
-      const bool in = row < left && c * 8 < D;
-      r[n] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, in ? (int)((unsigned)row * (unsigned)st * 2u + c * 16) : -16, 0, 0));
+      const int r = (wave * N + n) * RPI + lane / CPR, c = (lane % CPR) ^ swz<DP>(r);
+      off[n] = c * 8 < D ? (unsigned)r * (unsigned)st * 2u + c * 16u : 0x80000000u;
     }
   }
-  DEV void store(unsigned char* lds, int tid, const u32x4 (&r)[N]) {
+  // tile t of the sequence into the 64 rows at `lds` (LDS byte address); all four waves take part
+  __device__ __forceinline__ void load(int t, unsigned lds, int wave) const {
+    const int left = rows - t * 64;
+    const uint64_t at = (uint64_t)(base + (int64_t)t * 64 * st);
+    const unsigned bytes = left <= 0 ? 0u : (unsigned)(min(left, 64) - 1) * (unsigned)st * 2u + (unsigned)D * 2u;
+    const u32x4 rs = {(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((int)((at >> 32) & 0xffff)),
+                      (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int x = tid + n * NT, row = x / CPR, c = x % CPR;
-      *reinterpret_cast<u32x4*>(lds + tile_at<DP>(row, c)) = r[n];
-    }
+    for (int n = 0; n < N; ++n)
+      asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   ::"{m0}"(lds + (unsigned)(wave * N + n) * 1024u), "v"(off[n]), "s"(rs)
+                   : "memory");
   }
 };
+DEV void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+DEV unsigned lds_addr(const void* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p; }
 
 // one lane's operand fragments of row `row` (piece 2 ks + hi), zeros where the row does not count
 template <int DP>
@@ -181,162 +193,164 @@ DEV void store4(uint16_t* p, float a, float b, float c, float d) {
 }
 
 // =============================================================================================== forward
-// One workgroup = 4 waves x 32 QW queries of one (sequence, head); 64-key tiles of K and V, double buffered in LDS.
-template <class E, int DP, int QW>
-__global__ __launch_bounds__(256, 2) void rb_fwd_kernel(RbArgs a) {
+// One workgroup = 4 waves x 32 queries of one (sequence, head); 64-key tiles of K and V, double buffered in LDS.
+template <class E, int DP>
+__global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   constexpr int P = 2 * DP, TILE = 64 * P, NK = DP / 16, ND = DP / 32;
   unsigned char* const sK = smem;
   unsigned char* const sV = smem + 2 * TILE;
   float* const sB = reinterpret_cast<float*>(smem + 4 * TILE);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, n32 = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const int id = xcd_order(blockIdx.x, a.nblk);
   const int bh = id / a.ntile, tile = a.ntile - 1 - id % a.ntile;  // a causal row's last tiles are the longest: first
   const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
   const Seq sq = seq_of(a, b);
-  const int q0 = tile * (128 * QW), p_first = sq.off + q0 + wave * 32 * QW;
-  const uint16_t* const kp = a.k + b * a.sk.b + hk * a.sk.h;
-  const uint16_t* const vp = a.v + b * a.sv.b + hk * a.sv.h;
-
-  int kend = q0 < sq.qlen ? sq.klen : 0, wend = q0 + wave * 32 * QW < sq.qlen ? sq.klen : 0;
+  const int q0 = tile * 128, i = q0 + wave * 32 + n32, p0 = sq.off + q0 + wave * 32;
+  int kend = q0 < sq.qlen ? sq.klen : 0, wend = q0 + wave * 32 < sq.qlen ? sq.klen : 0;
   if (a.causal) {
-    kend = min(kend, sq.off + min(q0 + 128 * QW, sq.qlen));
-    wend = min(wend, p_first + 32 * QW);
+    kend = min(kend, sq.off + min(q0 + 128, sq.qlen));
+    wend = min(wend, p0 + 32);
   }
   const int nt = kend > 0 ? (kend + 63) >> 6 : 0;
 
-  Stage<DP, 256> lk, lv;
+  TileDma<DP> dk, dv;
+  dk.init(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, sq.klen, a.D, wave, lane);
+  dv.init(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, sq.klen, a.D, wave, lane);
+  const unsigned lK = lds_addr(sK), lV = lds_addr(sV);
   if (nt > 0) {
-    lk.load(kp, a.sk.t, 0, sq.klen, a.D, tid, lk.r);
-    lv.load(vp, a.sv.t, 0, sq.klen, a.D, tid, lv.r);
+    dk.load(0, lK, wave);
+    dv.load(0, lV, wave);
   }
-  u32x4 qf[QW][NK];
-  f32x16 o[QW][ND];
-  float m[QW], l[QW];
+  u32x4 qf[NK];
+  f32x16 o[ND];
+  float m = -RB_INF, l = 0.f;
+  row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, i, i < sq.qlen, a.D, hi, qf);
 #pragma unroll
-  for (int w = 0; w < QW; ++w) {
-    const int i = q0 + (wave * QW + w) * 32 + n32;
-    row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, i, i < sq.qlen, a.D, hi, qf[w]);
-    m[w] = -RB_INF;
-    l[w] = 0.f;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) o[w][d] = splat16(0.f);
-  }
+  for (int d = 0; d < ND; ++d) o[d] = splat16(0.f);
   spread_table(a, h, sB, tid, 256);
-  if (nt > 0) {
-    lk.store(sK, tid, lk.r);
-    lv.store(sV, tid, lv.r);
-  }
+  dma_wait();
   __syncthreads();
   const float left = sB[0], right = sB[2 * (a.md + RB_PAD)];
 
   for (int t = 0; t < nt; ++t) {
-    const int j0 = t * 64;
-    const bool more = t + 1 < nt;
-    if (more) {
-      lk.load(kp, a.sk.t, j0 + 64, sq.klen, a.D, tid, lk.r);
-      lv.load(vp, a.sv.t, j0 + 64, sq.klen, a.D, tid, lv.r);
+    const int j0 = t * 64, buf = t & 1;
+    if (t + 1 < nt) {
+      dk.load(t + 1, lK + (buf ^ 1) * TILE, wave);
+      dv.load(t + 1, lV + (buf ^ 1) * TILE, wave);
     }
-    const unsigned char* const kt = sK + (t & 1) * TILE;
-    const unsigned char* const vt = sV + (t & 1) * TILE;
     if (j0 < wend) {
-      f32x16 s[QW][2];
+      const unsigned char* const kt = sK + buf * TILE;
+      const unsigned char* const vt = sV + buf * TILE;
+      f32x16 s[2];
+      // far tiles: the bias is a constant, added with the running reference
+      const bool far = j0 - (p0 + 31) >= a.md || j0 + 63 - p0 <= -a.md;
+      const float cb = far ? (j0 > p0 ? right : left) : 0.f;
+      if (far) {
+        s[0] = s[1] = splat16(0.f);
+      } else {
+        const float* const bp = sB + (j0 - p0 - n32 + 4 * hi + a.md + RB_PAD);
 #pragma unroll
-      for (int w = 0; w < QW; ++w) {
-        const int p0 = p_first + 32 * w;
-        if (j0 - (p0 + 31) >= a.md || j0 + 63 - p0 <= -a.md) {
-          s[w][0] = s[w][1] = splat16(j0 > p0 ? right : left);
-        } else {
-          const float* const bp = sB + (j0 - p0 - n32 + 4 * hi + a.md + RB_PAD);
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[w][u][r] = bp[32 * u + 8 * (r >> 2) + (r & 3)];
-        }
+          for (int r = 0; r < 16; ++r) s[u][r] = bp[32 * u + 8 * (r >> 2) + (r & 3)];
       }
+      // operands are requested in groups ahead of the products that use them: left alone, the compiler reads, waits and
+      // multiplies one fragment at a time
+      constexpr int GK = 4;
+      u32x4 kf[GK][2];
 #pragma unroll
-      for (int ks = 0; ks < NK; ++ks)
+      for (int k0 = 0; k0 < NK; k0 += GK) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const u32x4 kf = frag<DP>(kt, 32 * u + n32, ks, hi);
+        for (int ks = 0; ks < GK && k0 + ks < NK; ++ks)
 #pragma unroll
-          for (int w = 0; w < QW; ++w) s[w][u] = E::mma(kf, qf[w][ks], s[w][u]);
-        }
-      u32x4 pb[QW][4];
+          for (int u = 0; u < 2; ++u) kf[ks][u] = frag<DP>(kt, 32 * u + n32, k0 + ks, hi);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int w = 0; w < QW; ++w) {
-        const int p0 = p_first + 32 * w;
-        if (j0 + 64 > sq.klen || (a.causal && j0 + 63 > p0)) {
-          const int lim = (a.causal ? min(sq.klen, p0 + n32 + 1) : sq.klen) - j0 - 4 * hi;
+        for (int ks = 0; ks < GK && k0 + ks < NK; ++ks)
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (32 * u + 8 * (r >> 2) + (r & 3) >= lim) s[w][u][r] = -RB_INF;
-        }
-        float mx = fmaxf(s[w][0][0], s[w][1][0]);
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx = fmaxf(fmaxf(mx, s[w][0][r]), s[w][1][r]);
-        mx = half_max(mx);
-        // the reference moves only when some row's scores outgrow it by 2^8: probabilities stay below 256 and the sums in f32
-        if (__any((mx - m[w]) * a.c2 > 8.f)) {
-          const float up = fmaxf(m[w], mx);
-          const float al = up == -RB_INF ? 1.f : __builtin_amdgcn_exp2f((m[w] - up) * a.c2);
-          m[w] = up;
-          l[w] *= al;
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[w][d][r] *= al;
-        }
-        const float mc = m[w] == -RB_INF ? 0.f : m[w] * a.c2;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            s[w][u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w][u][r], a.c2, -mc));
-            l[w] += s[w][u][r];
-          }
-          pb[w][2 * u] = pack8<E>(s[w][u], 0);
-          pb[w][2 * u + 1] = pack8<E>(s[w][u], 8);
-        }
+          for (int u = 0; u < 2; ++u) s[u] = E::mma(kf[ks][u], qf[k0 + ks], s[u]);
       }
+      u32x4 vf[2][ND];
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
+      for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const u32x4 vf = frag_t<DP>(vt, 16 * kk, d, lane);
+        for (int d = 0; d < ND; ++d) vf[kk][d] = frag_t<DP>(vt, 16 * kk, d, lane);
+      __builtin_amdgcn_sched_barrier(0);
+      if (j0 + 64 > sq.klen || (a.causal && j0 + 63 > p0)) {
+        const int lim = (a.causal ? min(sq.klen, p0 + n32 + 1) : sq.klen) - j0 - 4 * hi;
 #pragma unroll
-          for (int w = 0; w < QW; ++w) o[w][d] = E::mma(vf, pb[w][kk], o[w][d]);
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (32 * u + 8 * (r >> 2) + (r & 3) >= lim) s[u][r] = -RB_INF;
+      }
+      float mx[2] = {fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])};
+#pragma unroll
+      for (int r = 2; r < 16; r += 2)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) mx[u] = fmaxf(fmaxf(mx[u], s[u][r]), s[u][r + 1]);
+      const float top = half_max(fmaxf(mx[0], mx[1])) + cb;
+      // the running reference moves only when some row's scores outgrow it by 2^8: probabilities stay below 256, the sums in f32
+      if (__any((top - m) * a.c2 > 8.f)) {
+        const float up = fmaxf(m, top);
+        const float al = up == -RB_INF ? 1.f : __builtin_amdgcn_exp2f((m - up) * a.c2);
+        m = up;
+        l *= al;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] *= al;
+      }
+      const float mc = ((m == -RB_INF ? 0.f : m) - cb) * a.c2;
+      u32x4 pb[4];
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], a.c2, -mc));
+          sum[u] += s[u][r];
         }
+        pb[2 * u] = pack8<E>(s[u], 0);
+        pb[2 * u + 1] = pack8<E>(s[u], 8);
+      }
+      l += sum[0] + sum[1];
+      u32x4 vg[2][ND];
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) vg[kk][d] = frag_t<DP>(vt, 32 + 16 * kk, d, lane);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] = E::mma(vf[kk][d], pb[kk], o[d]);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] = E::mma(vg[kk][d], pb[2 + kk], o[d]);
     }
-    if (more) {
-      lk.store(sK + ((t + 1) & 1) * TILE, tid, lk.r);
-      lv.store(sV + ((t + 1) & 1) * TILE, tid, lv.r);
-    }
+    dma_wait();
     __syncthreads();
   }
 
+  if (i >= a.Tq) return;
+  const float all = half_sum(l);
+  const float sum = i < sq.qlen ? all : 0.f;  // rows behind the sequence and rows without keys: zeros, and -inf
+  const float inv = 1.f / sum;
+  uint16_t* const op = a.out + b * a.so.b + (int64_t)i * a.so.t + h * a.so.h;
 #pragma unroll
-  for (int w = 0; w < QW; ++w) {
-    const int i = q0 + (wave * QW + w) * 32 + n32;
-    if (i >= a.Tq) continue;
-    const float all = half_sum(l[w]);
-    const float sum = i < sq.qlen ? all : 0.f;  // rows behind the sequence and rows without keys: zeros, and -inf
-    const float inv = 1.f / sum;
-    uint16_t* const op = a.out + b * a.so.b + (int64_t)i * a.so.t + h * a.so.h;
+  for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int c = 32 * d + 8 * g + 4 * hi;
-        if (c >= a.D) continue;
-        if (sum == 0.f) store4<E>(op + c, 0.f, 0.f, 0.f, 0.f);
-        else store4<E>(op + c, o[w][d][4 * g] * inv, o[w][d][4 * g + 1] * inv, o[w][d][4 * g + 2] * inv, o[w][d][4 * g + 3] * inv);
-      }
-    if (a.lse != nullptr && hi == 0)
-      a.lse[((int64_t)b * a.H + h) * a.Tq + i] = sum == 0.f ? -RB_INF : (m[w] * a.c2 + __builtin_amdgcn_logf(sum)) * RB_LN2;
-  }
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * d + 8 * g + 4 * hi;
+      if (c >= a.D) continue;
+      if (sum == 0.f) store4<E>(op + c, 0.f, 0.f, 0.f, 0.f);
+      else store4<E>(op + c, o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv);
+    }
+  if (a.lse != nullptr && hi == 0)
+    a.lse[((int64_t)b * a.H + h) * a.Tq + i] = sum == 0.f ? -RB_INF : (m * a.c2 + __builtin_amdgcn_logf(sum)) * RB_LN2;
 }
 
 // ------------------------------------------------------------------------------------ forward, few query rows
@@ -590,14 +604,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dq_kernel(RbArgs a)
   const int span = 2 * (a.md + RB_PAD) + 1;
   float* const sG = sB + span;                                      // [4 groups][2 halves][span]
   double* const sFar = reinterpret_cast<double*>(smem + 4 * TILE + ((9 * span + 1) / 2 * 2) * 4);  // [4][2]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, n32 = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const int id = xcd_order(blockIdx.x, a.nblk);
   const int bh = id / a.ntile, tile = a.ntile - 1 - id % a.ntile;
   const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
   const Seq sq = seq_of(a, b);
   const int q0 = tile * 128, i = q0 + wave * 32 + n32, p0 = sq.off + q0 + wave * 32;
-  const uint16_t* const kp = a.k + b * a.sk.b + hk * a.sk.h;
-  const uint16_t* const vp = a.v + b * a.sv.b + hk * a.sv.h;
   int kend = q0 < sq.qlen ? sq.klen : 0, wend = q0 + wave * 32 < sq.qlen ? sq.klen : 0;
   if (a.causal) {
     kend = min(kend, sq.off + min(q0 + 128, sq.qlen));
@@ -605,10 +617,13 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dq_kernel(RbArgs a)
   }
   const int nt = kend > 0 ? (kend + 63) >> 6 : 0;
 
-  Stage<DP, 256> lk, lv;
+  TileDma<DP> dK, dV;
+  dK.init(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, sq.klen, a.D, wave, lane);
+  dV.init(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, sq.klen, a.D, wave, lane);
+  const unsigned lK = lds_addr(sK), lV = lds_addr(sV);
   if (nt > 0) {
-    lk.load(kp, a.sk.t, 0, sq.klen, a.D, tid, lk.r);
-    lv.load(vp, a.sv.t, 0, sq.klen, a.D, tid, lv.r);
+    dK.load(0, lK, wave);
+    dV.load(0, lV, wave);
   }
   u32x4 qf[NK], df[NK];
   row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, i, i < sq.qlen, a.D, hi, qf);
@@ -625,7 +640,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dq_kernel(RbArgs a)
       for (int e = 0; e < 4; ++e) delta += E::lo(df[ks][e]) * E::lo(of[ks][e]) + E::hi(df[ks][e]) * E::hi(of[ks][e]);
     delta = half_sum(delta);
     if (x != -RB_INF) lse2 = x * RB_LOG2E;
-    if (hi == 0 && i < a.Tq) a.delta[at] = delta, a.lse2[at] = lse2;
+    const int64_t to = ((int64_t)b * a.H + h) * a.tq128 + i;  // rows up to the tile's end: the next kernel reads whole tiles
+    if (hi == 0) a.delta[to] = -delta, a.lse2[to] = lse2;
   }
   f32x16 dq[ND];
 #pragma unroll
@@ -635,10 +651,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dq_kernel(RbArgs a)
   bool pending = false;
   spread_table(a, h, sB, tid, 256);
   for (int x = tid; x < 8 * span; x += 256) sG[x] = 0.f;
-  if (nt > 0) {
-    lk.store(sK, tid, lk.r);
-    lv.store(sV, tid, lv.r);
-  }
+  dma_wait();
   __syncthreads();
   const float left = sB[0], right = sB[span - 1];
   // lane's cell for key base 0: its own class (half), or for lanes 0..2 the other half's, 32 keys before
@@ -646,10 +659,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dq_kernel(RbArgs a)
 
   for (int t = 0; t < nt; ++t) {
     const int j0 = t * 64;
-    const bool more = t + 1 < nt;
-    if (more) {
-      lk.load(kp, a.sk.t, j0 + 64, sq.klen, a.D, tid, lk.r);
-      lv.load(vp, a.sv.t, j0 + 64, sq.klen, a.D, tid, lv.r);
+    if (t + 1 < nt) {
+      dK.load(t + 1, lK + ((t + 1) & 1) * TILE, wave);
+      dV.load(t + 1, lV + ((t + 1) & 1) * TILE, wave);
     }
     const unsigned char* const kt = sK + (t & 1) * TILE;
     const unsigned char* const vt = sV + (t & 1) * TILE;
@@ -719,10 +731,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dq_kernel(RbArgs a)
         for (int d = 0; d < ND; ++d) dq[d] = E::mma(frag_t<DP>(kt, 32 * u + 16 * kk, d, lane), ds, dq[d]);
       }
     }
-    if (more) {
-      lk.store(sK + ((t + 1) & 1) * TILE, tid, lk.r);
-      lv.store(sV + ((t + 1) & 1) * TILE, tid, lv.r);
-    }
+    dma_wait();
     __syncthreads();
   }
   if (pending) {
@@ -790,16 +799,16 @@ DEV void table_sum(const RbArgs& a, int entry, int nwg) {
 template <class E, int DP>
 __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  if ((int)blockIdx.x >= a.nblk) {  // the last workgroups: the table's gradient from the dq kernel's shares
-    table_sum(a, (blockIdx.x - a.nblk) * 4 + (threadIdx.x >> 6), a.B * a.nqtile);
+  if ((int)blockIdx.x >= a.nblk) {  // more table entries than waves (few keys)
+    table_sum(a, blockIdx.x * 4 + (threadIdx.x >> 6), a.B * a.nqtile);
     return;
   }
   constexpr int P = 2 * DP, TILE = 64 * P, NK = DP / 16, ND = DP / 32;
   unsigned char* const sQ = smem;
   unsigned char* const sO = smem + 2 * TILE;
-  float* const sL = reinterpret_cast<float*>(smem + 4 * TILE);  // [2][2][64] lse2 | -delta
+  float* const sL = reinterpret_cast<float*>(smem + 4 * TILE);  // [2][2][64] lse2 | -delta of a tile's rows
   float* const sB = sL + 256;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, n32 = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const int id = xcd_order(blockIdx.x, a.nblk);
   const int bh = id / a.ntile, tile = id % a.ntile;
   const int b = bh / a.Hk, hk = bh % a.Hk, G = a.H / a.Hk;
@@ -814,37 +823,34 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
   // causal: the first query that sees key k0 sits at position k0
   const int t0 = a.causal ? max(k0 - sq.off, 0) >> 6 : 0;
   const int t1 = k0 < sq.klen ? (sq.qlen + 63) >> 6 : 0;
-  Stage<DP, 256> lq, lo;
+  const unsigned lQ = lds_addr(sQ), lO = lds_addr(sO);
   float lrow = 0.f;
 
   for (int g = 0; g < G; ++g) {
     const int h = hk * G + g;
-    const uint16_t* const qp = a.q + b * a.sq.b + h * a.sq.h;
-    const uint16_t* const dp_ = a.dout + b * a.sdo.b + h * a.sdo.h;
-    const float* const rl = a.lse2 + ((int64_t)b * a.H + h) * a.Tq;
-    const float* const rd = a.delta + ((int64_t)b * a.H + h) * a.Tq;
-    auto load = [&](int t) {
-      lq.load(qp, a.sq.t, t * 64, sq.qlen, a.D, tid, lq.r);
-      lo.load(dp_, a.sdo.t, t * 64, sq.qlen, a.D, tid, lo.r);
-      const int i = t * 64 + lane;
-      if (wave == 0) lrow = i < sq.qlen ? rl[i] : RB_INF;
-      else if (wave == 1) lrow = i < sq.qlen ? -rd[i] : 0.f;
+    TileDma<DP> dQ, dO;
+    dQ.init(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, sq.qlen, a.D, wave, lane);
+    dO.init(a.dout + b * a.sdo.b + h * a.sdo.h, a.sdo.t, sq.qlen, a.D, wave, lane);
+    const float* const rl = (wave == 0 ? a.lse2 : a.delta) + ((int64_t)b * a.H + h) * a.tq128;
+    auto load = [&](int t, int buf) {
+      dQ.load(t, lQ + buf * TILE, wave);
+      dO.load(t, lO + buf * TILE, wave);
+      if (wave < 2) lrow = rl[t * 64 + lane];
     };
     auto store = [&](int buf) {
-      lq.store(sQ + buf * TILE, tid, lq.r);
-      lo.store(sO + buf * TILE, tid, lo.r);
       if (wave < 2) sL[buf * 128 + wave * 64 + lane] = lrow;
     };
-    if (t0 < t1) load(t0);
     __syncthreads();  // the head before has been read
+    if (t0 < t1) load(t0, 0);
     spread_table(a, h, sB, tid, 256);
     if (t0 < t1) store(0);
+    dma_wait();
     __syncthreads();
     const float left = sB[0], right = sB[2 * (a.md + RB_PAD)];
     for (int t = t0; t < t1; ++t) {
       const int buf = (t - t0) & 1;
       const bool more = t + 1 < t1;
-      if (more) load(t + 1);
+      if (more) load(t + 1, buf ^ 1);
       const unsigned char* const qt = sQ + buf * TILE;
       const unsigned char* const ot = sO + buf * TILE;
       const float* const lt = sL + buf * 128;
@@ -895,9 +901,11 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
         }
       }
       if (more) store(buf ^ 1);
+      dma_wait();
       __syncthreads();
     }
   }
+  table_sum(a, blockIdx.x * 4 + wave, a.B * a.nqtile);  // each wave one entry of the table's gradient, from the dq kernel's shares
   if (j >= a.Tk) return;
   const bool in = j < sq.klen;  // rows behind the sequence get zeros
   uint16_t* const kp = a.dk + b * a.sdk.b + (int64_t)j * a.sdk.t + hk * a.sdk.h;
@@ -917,9 +925,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
 }
 
 // =============================================================================================== host side
-bool strides_ok(const int64_t* s) {
-  // 16-byte rows; a tile of 64 rows must stay within a 31-bit byte offset
-  return s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0 && s[1] >= 0 && s[1] < (1 << 23) && s[0] >= 0 && s[2] >= 0;
+bool strides_ok(const int64_t* s, int D) {
+  // 16-byte rows that do not overlap; a tile of 64 rows must stay within a 31-bit byte offset
+  return s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0 && s[1] >= D && s[1] < (1 << 23) && s[0] >= 0 && s[2] >= 0;
 }
 Strides to_strides(const int64_t* s) { return Strides{s[0], s[1], s[2]}; }
 
@@ -937,7 +945,7 @@ int check_args(const csship_relbias* p) {
   const bool rows = p->B > 0 && p->Tq > 0, keys = p->B > 0 && p->Tk > 0;
   if ((rows && p->q == nullptr) || (keys && (p->k == nullptr || p->v == nullptr))) return CSSHIP_ENULL;
   if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v)) return CSSHIP_EALIGN;
-  if (!strides_ok(p->q_stride) || !strides_ok(p->k_stride) || !strides_ok(p->v_stride)) return CSSHIP_EALIGN;
+  if (!strides_ok(p->q_stride, p->D) || !strides_ok(p->k_stride, p->D) || !strides_ok(p->v_stride, p->D)) return CSSHIP_EALIGN;
   return CSSHIP_OK;
 }
 
@@ -997,18 +1005,20 @@ int launch_fwd(RbArgs a, const csship_relbias* p, hipStream_t s) {
   a.ntile = (a.Tq + 127) / 128;
   a.nblk = a.B * a.H * a.ntile;
   if (a.nblk == 0) return CSSHIP_OK;
-  return launch(rb_fwd_kernel<E, DP, 1>, a.nblk, fwd_lds(DP, a.md), a, s);
+  return launch(rb_fwd_kernel<E, DP>, a.nblk, fwd_lds(DP, a.md), a, s);
 }
 
 template <class E, int DP>
 int launch_bwd(RbArgs a, hipStream_t s) {
   a.ntile = a.nqtile = (a.Tq + 127) / 128;
+  a.tq128 = a.ntile * 128;
   a.nblk = a.B * a.H * a.ntile;
   if (a.nblk > 0)
     if (const int rc = launch(rb_dq_kernel<E, DP>, a.nblk, dq_lds(DP, a.md), a, s)) return rc;
   a.ntile = (a.Tk + 127) / 128;
   a.nblk = a.B * a.Hk * a.ntile;
-  return launch(rb_dkv_kernel<E, DP>, (int64_t)a.nblk + (a.nb * a.H + 3) / 4, dkv_lds(DP, a.md), a, s);
+  const int64_t entries = ((int64_t)a.nb * a.H + 3) / 4;
+  return launch(rb_dkv_kernel<E, DP>, a.nblk > entries ? a.nblk : entries, dkv_lds(DP, a.md), a, s);
 }
 
 template <class E>
@@ -1020,7 +1030,7 @@ int bwd_by_width(const RbArgs& a, hipStream_t s) {
   return a.D <= 32 ? launch_bwd<E, 32>(a, s) : a.D <= 64 ? launch_bwd<E, 64>(a, s) : launch_bwd<E, 128>(a, s);
 }
 
-int64_t row_words(const csship_relbias* p) { return ((int64_t)p->B * p->H * p->Tq + 3) / 4 * 4; }
+int64_t row_words(const csship_relbias* p) { return (int64_t)p->B * p->H * ((p->Tq + 127) / 128 * 128); }
 
 }  // namespace
 
@@ -1041,7 +1051,7 @@ int csship_relbias_fwd(const csship_relbias* p, uint16_t* out, const int64_t* ou
   if (!aligned16(workspace)) return CSSHIP_EALIGN;
   if (p->B == 0 || p->Tq == 0) return CSSHIP_OK;
   if (out == nullptr || out_stride == nullptr) return CSSHIP_ENULL;
-  if (!aligned8(out) || !strides_ok(out_stride)) return CSSHIP_EALIGN;
+  if (!aligned8(out) || !strides_ok(out_stride, p->D)) return CSSHIP_EALIGN;
   RbArgs a = to_args(p);
   a.out = out;
   a.so = to_strides(out_stride);
@@ -1068,7 +1078,7 @@ int csship_relbias_bwd(const csship_relbias* p, const uint16_t* out, const int64
   if ((rows && (out == nullptr || lse == nullptr || dout == nullptr || dq == nullptr)) || (keys && (dk == nullptr || dv == nullptr)))
     return CSSHIP_ENULL;
   if (!aligned16(out) || !aligned16(dout) || !aligned8(dq) || !aligned8(dk) || !aligned8(dv) || !aligned16(workspace)) return CSSHIP_EALIGN;
-  if (!strides_ok(out_stride) || !strides_ok(dout_stride) || !strides_ok(dq_stride) || !strides_ok(dk_stride) || !strides_ok(dv_stride))
+  if (!strides_ok(out_stride, p->D) || !strides_ok(dout_stride, p->D) || !strides_ok(dq_stride, p->D) || !strides_ok(dk_stride, p->D) || !strides_ok(dv_stride, p->D))
     return CSSHIP_EALIGN;
   if (workspace_bytes < csship_relbias_bwd_workspace(p)) return CSSHIP_EWORKSPACE;
   RbArgs a = to_args(p);

@@ -335,7 +335,7 @@ def _relbias_rows(t, name, like=None):
             raise TypeError(f"css_amd: '{name}' must be {like.dtype}, got {dt}")
         if t.get_device() != like.get_device():
             raise RuntimeError(f"css_amd: '{name}' is on {t.device}, the queries on {like.device}")
-    if s[3] != 1 or (s[0] | s[1] | s[2]) & 7 or s[1] >= 1 << 23 or t.data_ptr() & 15:
+    if s[3] != 1 or (s[0] | s[1] | s[2]) & 7 or not t.shape[3] <= s[1] < 1 << 23 or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 

@@ -1148,7 +1148,7 @@ void csship_debug_stamps(void* device_buffer);
  *   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,  dv_j = sum_i P_ij dout_i  (sums over the heads of the group),
  *   dtable[n, h] = sum of dS_ij over the pairs with bucket(r) = n, over all sequences
  * q, out, dout, dq [B, Tq, H, D]; k, v, dk, dv [B, Tk, Hk, D], bf16 or fp16 (dtype), strides in ELEMENTS for (sequence, frame,
- * head), the last dimension dense; strides are non-negative multiples of 8, the frame stride below 2^23, inputs 16-byte and
+ * head), the last dimension dense; strides are non-negative multiples of 8, the frame stride from D to below 2^23, inputs 16-byte and
  * results 8-byte aligned.  D is a multiple of 8 up to 128.  lse f32 [B, H, Tq] dense.  table, dtable f32 [n_buckets, H] dense.
  * bucket_of int16 [2 max_distance + 1]: the bucket of r at bucket_of[r + max_distance]; distances beyond +-max_distance take the
  * end entries.  bucket_range int32 [n_buckets][2] (backward): bucket n holds the distances bucket_range[n][0] <= r <
