@@ -28,6 +28,11 @@ constexpr float RB_BIG = 1048576.f; // table entries at or below -2^20 ban their
 constexpr int RB_MAX_POS = 1 << 28;  // lengths and offsets stay below it: distances in 32 bits
 constexpr float RB_INF = __builtin_inff();
 
+template <int N>
+struct Const { static constexpr int value = N; };
+using True = Const<1>;
+using False = Const<0>;
+
 struct ElemBf {
   DEV f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -125,29 +130,30 @@ template <int DP>
 struct TileDma {
   static constexpr int CPR = DP / 8, RPI = 64 / CPR, N = 16 / RPI;  // pieces a row, rows an instruction, instructions a wave
   unsigned off[N];
-  const uint16_t* base;
-  int64_t st;
-  int rows, D;
-  __device__ __forceinline__ void init(const uint16_t* b, int64_t stride, int rows_, int D_, int wave, int lane) {
-    base = b, st = stride, rows = rows_, D = D_;
+  uint64_t at;    // address of the next tile
+  int64_t left;   // bytes from there to the end of the last row, 0 and less: none
+  unsigned step;  // bytes of 64 rows
+  __device__ __forceinline__ void init(const uint16_t* base, int64_t stride, int tile, int rows, int D, int wave, int lane) {
+    step = (unsigned)stride * 128u;
+    at = (uint64_t)(base + (int64_t)tile * 64 * stride);
+    left = rows > 0 ? ((int64_t)(rows - 1) * stride + D) * 2 - (int64_t)tile * step : 0;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int r = (wave * N + n) * RPI + lane / CPR, c = (lane % CPR) ^ swz<DP>(r);
-      off[n] = c * 8 < D ? (unsigned)r * (unsigned)st * 2u + c * 16u : 0x80000000u;
+      off[n] = c * 8 < D ? (unsigned)r * (unsigned)stride * 2u + c * 16u : 0xfffffff0u;
     }
   }
-  // tile t of the sequence into the 64 rows at `lds` (LDS byte address); all four waves take part
-  __device__ __forceinline__ void load(int t, unsigned lds, int wave) const {
-    const int left = rows - t * 64;
-    const uint64_t at = (uint64_t)(base + (int64_t)t * 64 * st);
-    const unsigned bytes = left <= 0 ? 0u : (unsigned)(min(left, 64) - 1) * (unsigned)st * 2u + (unsigned)D * 2u;
-    const u32x4 rs = {(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((int)((at >> 32) & 0xffff)),
-                      (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+  // the next 64 rows to LDS byte address `lds`; all four waves take part
+  __device__ __forceinline__ void next(unsigned lds, int wave) {
+    const u32x4 rs = {(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((int)(at >> 32)) & 0xffffu,
+                      (unsigned)__builtin_amdgcn_readfirstlane((int)(left <= 0 ? 0u : left < (int64_t)step ? (unsigned)left : step)), 0x00020000u};
 #pragma unroll
     for (int n = 0; n < N; ++n)
       asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                    ::"{m0}"(lds + (unsigned)(wave * N + n) * 1024u), "v"(off[n]), "s"(rs)
                    : "memory");
+    at += step;
+    left -= step;
   }
 };
 DEV void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
@@ -192,6 +198,26 @@ DEV void store4(uint16_t* p, float a, float b, float c, float d) {
   *reinterpret_cast<uint2*>(p) = make_uint2(E::pack(a, b), E::pack(c, d));
 }
 
+// a wave's 32 finished rows: out = O / sum, log-sum-exp; rows behind the sequence and rows without keys: zeros, and -inf
+template <class E, int DP>
+DEV void store_rows(const RbArgs& a, const f32x16 (&o)[DP / 32], float m, float l, int b, int h, int i, int hi, bool valid) {
+  const float all = half_sum(l);
+  if (i >= a.Tq) return;
+  const float sum = valid ? all : 0.f, inv = 1.f / sum;
+  uint16_t* const op = a.out + b * a.so.b + (int64_t)i * a.so.t + h * a.so.h;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * d + 8 * g + 4 * hi;
+      if (c >= a.D) continue;
+      if (sum == 0.f) store4<E>(op + c, 0.f, 0.f, 0.f, 0.f);
+      else store4<E>(op + c, o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv);
+    }
+  if (a.lse != nullptr && hi == 0)
+    a.lse[((int64_t)b * a.H + h) * a.Tq + i] = sum == 0.f ? -RB_INF : (m * a.c2 + __builtin_amdgcn_logf(sum)) * RB_LN2;
+}
+
 // =============================================================================================== forward
 // One workgroup = 4 waves x 32 queries of one (sequence, head); 64-key tiles of K and V, double buffered in LDS.
 template <class E, int DP>
@@ -215,12 +241,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
   const int nt = kend > 0 ? (kend + 63) >> 6 : 0;
 
   TileDma<DP> dk, dv;
-  dk.init(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, sq.klen, a.D, wave, lane);
-  dv.init(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, sq.klen, a.D, wave, lane);
+  dk.init(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, 0, sq.klen, a.D, wave, lane);
+  dv.init(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, 0, sq.klen, a.D, wave, lane);
   const unsigned lK = lds_addr(sK), lV = lds_addr(sV);
   if (nt > 0) {
-    dk.load(0, lK, wave);
-    dv.load(0, lV, wave);
+    dk.next(lK, wave);
+    dv.next(lV, wave);
   }
   u32x4 qf[NK];
   f32x16 o[ND];
@@ -233,43 +259,48 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
   __syncthreads();
   const float left = sB[0], right = sB[2 * (a.md + RB_PAD)];
 
-  for (int t = 0; t < nt; ++t) {
-    const int j0 = t * 64, buf = t & 1;
+  // one tile; the buffer's parity is a constant (LDS addresses are then lane addresses and immediates)
+  auto step = [&](int t, auto parity) {
+    constexpr int buf = decltype(parity)::value;
+    const int j0 = t * 64;
     if (t + 1 < nt) {
-      dk.load(t + 1, lK + (buf ^ 1) * TILE, wave);
-      dv.load(t + 1, lV + (buf ^ 1) * TILE, wave);
+      dk.next(lK + (buf ^ 1) * TILE, wave);
+      dv.next(lV + (buf ^ 1) * TILE, wave);
     }
     if (j0 < wend) {
       const unsigned char* const kt = sK + buf * TILE;
       const unsigned char* const vt = sV + buf * TILE;
       f32x16 s[2];
+      // S^T = K Q^T + bias.  Operands are requested in groups ahead of the products that use them: left alone, the compiler
+      // reads, waits and multiplies one fragment at a time.
+      auto scores = [&](auto zero) {
+        constexpr int GK = 4;
+        u32x4 kf[GK][2];
+#pragma unroll
+        for (int k0 = 0; k0 < NK; k0 += GK) {
+#pragma unroll
+          for (int ks = 0; ks < GK && k0 + ks < NK; ++ks)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) kf[ks][u] = frag<DP>(kt, 32 * u + n32, k0 + ks, hi);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int ks = 0; ks < GK && k0 + ks < NK; ++ks)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) s[u] = E::mma(kf[ks][u], qf[k0 + ks], decltype(zero)::value && k0 + ks == 0 ? splat16(0.f) : s[u]);
+        }
+      };
       // far tiles: the bias is a constant, added with the running reference
       const bool far = j0 - (p0 + 31) >= a.md || j0 + 63 - p0 <= -a.md;
       const float cb = far ? (j0 > p0 ? right : left) : 0.f;
       if (far) {
-        s[0] = s[1] = splat16(0.f);
+        scores(True{});
       } else {
         const float* const bp = sB + (j0 - p0 - n32 + 4 * hi + a.md + RB_PAD);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[u][r] = bp[32 * u + 8 * (r >> 2) + (r & 3)];
-      }
-      // operands are requested in groups ahead of the products that use them: left alone, the compiler reads, waits and
-      // multiplies one fragment at a time
-      constexpr int GK = 4;
-      u32x4 kf[GK][2];
-#pragma unroll
-      for (int k0 = 0; k0 < NK; k0 += GK) {
-#pragma unroll
-        for (int ks = 0; ks < GK && k0 + ks < NK; ++ks)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) kf[ks][u] = frag<DP>(kt, 32 * u + n32, k0 + ks, hi);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int ks = 0; ks < GK && k0 + ks < NK; ++ks)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) s[u] = E::mma(kf[ks][u], qf[k0 + ks], s[u]);
+        scores(False{});
       }
       u32x4 vf[2][ND];
 #pragma unroll
@@ -333,24 +364,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
     }
     dma_wait();
     __syncthreads();
+  };
+  for (int t = 0; t < nt; t += 2) {
+    step(t, Const<0>{});
+    if (t + 1 < nt) step(t + 1, Const<1>{});
   }
-
-  if (i >= a.Tq) return;
-  const float all = half_sum(l);
-  const float sum = i < sq.qlen ? all : 0.f;  // rows behind the sequence and rows without keys: zeros, and -inf
-  const float inv = 1.f / sum;
-  uint16_t* const op = a.out + b * a.so.b + (int64_t)i * a.so.t + h * a.so.h;
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int c = 32 * d + 8 * g + 4 * hi;
-      if (c >= a.D) continue;
-      if (sum == 0.f) store4<E>(op + c, 0.f, 0.f, 0.f, 0.f);
-      else store4<E>(op + c, o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv);
-    }
-  if (a.lse != nullptr && hi == 0)
-    a.lse[((int64_t)b * a.H + h) * a.Tq + i] = sum == 0.f ? -RB_INF : (m * a.c2 + __builtin_amdgcn_logf(sum)) * RB_LN2;
+  store_rows<E, DP>(a, o, m, l, b, h, i, hi, i < sq.qlen);
 }
 
 // ------------------------------------------------------------------------------------ forward, few query rows
@@ -618,12 +637,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dq_kernel(RbArgs a)
   const int nt = kend > 0 ? (kend + 63) >> 6 : 0;
 
   TileDma<DP> dK, dV;
-  dK.init(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, sq.klen, a.D, wave, lane);
-  dV.init(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, sq.klen, a.D, wave, lane);
+  dK.init(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, 0, sq.klen, a.D, wave, lane);
+  dV.init(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, 0, sq.klen, a.D, wave, lane);
   const unsigned lK = lds_addr(sK), lV = lds_addr(sV);
   if (nt > 0) {
-    dK.load(0, lK, wave);
-    dV.load(0, lV, wave);
+    dK.next(lK, wave);
+    dV.next(lV, wave);
   }
   u32x4 qf[NK], df[NK];
   row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, i, i < sq.qlen, a.D, hi, qf);
@@ -660,8 +679,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dq_kernel(RbArgs a)
   for (int t = 0; t < nt; ++t) {
     const int j0 = t * 64;
     if (t + 1 < nt) {
-      dK.load(t + 1, lK + ((t + 1) & 1) * TILE, wave);
-      dV.load(t + 1, lV + ((t + 1) & 1) * TILE, wave);
+      dK.next(lK + ((t + 1) & 1) * TILE, wave);
+      dV.next(lV + ((t + 1) & 1) * TILE, wave);
     }
     const unsigned char* const kt = sK + (t & 1) * TILE;
     const unsigned char* const vt = sV + (t & 1) * TILE;
@@ -829,12 +848,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
   for (int g = 0; g < G; ++g) {
     const int h = hk * G + g;
     TileDma<DP> dQ, dO;
-    dQ.init(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, sq.qlen, a.D, wave, lane);
-    dO.init(a.dout + b * a.sdo.b + h * a.sdo.h, a.sdo.t, sq.qlen, a.D, wave, lane);
+    dQ.init(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, t0, sq.qlen, a.D, wave, lane);
+    dO.init(a.dout + b * a.sdo.b + h * a.sdo.h, a.sdo.t, t0, sq.qlen, a.D, wave, lane);
     const float* const rl = (wave == 0 ? a.lse2 : a.delta) + ((int64_t)b * a.H + h) * a.tq128;
     auto load = [&](int t, int buf) {
-      dQ.load(t, lQ + buf * TILE, wave);
-      dO.load(t, lO + buf * TILE, wave);
+      dQ.next(lQ + buf * TILE, wave);
+      dO.next(lO + buf * TILE, wave);
       if (wave < 2) lrow = rl[t * 64 + lane];
     };
     auto store = [&](int buf) {
