@@ -65,8 +65,8 @@ struct RbArgs {
   uint16_t *out, *dq, *dk, *dv;
   float *lse, *dtable;
   const float* lse_in;
-  float *delta, *lse2, *part;  // workspace; delta (negated) and lse2 [B, H, tq128]
-  int B, Tq, Tk, H, Hk, D, nb, md, causal, offset;
+  float *delta, *lse2, *part, *part2;  // workspace; delta (negated) and lse2 [B, H, tq128]
+  int B, Tq, Tk, H, Hk, D, nb, md, mde, causal, offset;  // mde: md, or the furthest distance that occurs
   float scale, inv_scale, c2;  // c2 = scale * log2(e)
   int ntile, nblk, nsplit, nqtile, tq128;     // row tiles per (sequence, head); workgroups; key ranges (rb_few_kernel)
 };
@@ -100,13 +100,32 @@ DEV int xcd_order(int id, int n) {
 }
 
 // table entry -> score units (the products' accumulators hold q . k, scaled later by c2)
-DEV float bias_entry(const RbArgs& a, int r, int h) {
-  const float w = a.table[a.bucket_of[r + a.md] * a.H + h];
-  return w <= -RB_BIG ? -RB_INF : (w > RB_BIG ? RB_BIG : w) * a.inv_scale;
-}
-DEV void spread_table(const RbArgs& a, int h, float* sB, int tid, int nthreads) {
-  const int n = 2 * (a.md + RB_PAD) + 1;
-  for (int i = tid; i < n; i += nthreads) sB[i] = bias_entry(a, min(max(i - a.md - RB_PAD, -a.md), a.md), h);
+DEV float bias_units(const RbArgs& a, float w) { return w <= -RB_BIG ? -RB_INF : (w > RB_BIG ? RB_BIG : w) * a.inv_scale; }
+DEV float bias_entry(const RbArgs& a, int r, int h) { return bias_units(a, a.table[a.bucket_of[r + a.md] * a.H + h]); }
+// A head's table by distance, -mde - RB_PAD .. mde + RB_PAD, in LDS; 256 threads, barriers inside.  The table's column goes
+// through `scratch` (`cap` floats), so that it and the bucket numbers are loaded side by side and not one behind the other.
+DEV void spread_table(const RbArgs& a, int h, float* sB, float* scratch, int cap, int tid) {
+  const int n = 2 * (a.mde + RB_PAD) + 1;
+  const bool staged = a.nb <= cap;
+  if (staged)
+    for (int i = tid; i < a.nb; i += 256) scratch[i] = bias_units(a, a.table[i * a.H + h]);
+  constexpr int AHEAD = 4;
+  int id[AHEAD];
+#pragma unroll
+  for (int e = 0; e < AHEAD; ++e) {
+    const int i = tid + e * 256;
+    id[e] = i < n ? a.bucket_of[min(max(i - a.mde - RB_PAD, -a.mde), a.mde) + a.md] : 0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < AHEAD; ++e) {
+    const int i = tid + e * 256;
+    if (i < n) sB[i] = staged ? scratch[id[e]] : bias_units(a, a.table[id[e] * a.H + h]);
+  }
+  for (int i = tid + AHEAD * 256; i < n; i += 256) {
+    const int x = a.bucket_of[min(max(i - a.mde - RB_PAD, -a.mde), a.mde) + a.md];
+    sB[i] = staged ? scratch[x] : bias_units(a, a.table[x * a.H + h]);
+  }
 }
 
 // over the two half waves (lanes l and l ^ 32), in both
@@ -254,10 +273,10 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
   row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, i, i < sq.qlen, a.D, hi, qf);
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = splat16(0.f);
-  spread_table(a, h, sB, tid, 256);
+  spread_table(a, h, sB, reinterpret_cast<float*>(sK + TILE), TILE / 4, tid);
   dma_wait();
   __syncthreads();
-  const float left = sB[0], right = sB[2 * (a.md + RB_PAD)];
+  const float left = sB[0], right = sB[2 * (a.mde + RB_PAD)];
 
   // one tile; the buffer's parity is a constant (LDS addresses are then lane addresses and immediates)
   auto step = [&](int t, auto parity) {
@@ -290,12 +309,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
         }
       };
       // far tiles: the bias is a constant, added with the running reference
-      const bool far = j0 - (p0 + 31) >= a.md || j0 + 63 - p0 <= -a.md;
+      const bool far = j0 - (p0 + 31) >= a.mde || j0 + 63 - p0 <= -a.mde;
       const float cb = far ? (j0 > p0 ? right : left) : 0.f;
       if (far) {
         scores(True{});
       } else {
-        const float* const bp = sB + (j0 - p0 - n32 + 4 * hi + a.md + RB_PAD);
+        const float* const bp = sB + (j0 - p0 - n32 + 4 * hi + a.mde + RB_PAD);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -614,13 +633,13 @@ DEV float swap_halves(float x) {
 // It also leaves delta_i = do_i . o_i and the rows' log-sum-exp in log2 units for the next kernel, +inf where a row has no
 // keys or lies behind its sequence (exp2(s - inf) = 0: such rows drop out of every product).
 template <class E, int DP>
-__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dq_kernel(RbArgs a) {
+__global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   constexpr int P = 2 * DP, TILE = 64 * P, NK = DP / 16, ND = DP / 32;
   unsigned char* const sK = smem;
   unsigned char* const sV = smem + 2 * TILE;
   float* const sB = reinterpret_cast<float*>(smem + 4 * TILE);
-  const int span = 2 * (a.md + RB_PAD) + 1;
+  const int span = 2 * (a.mde + RB_PAD) + 1;
   float* const sG = sB + span;                                      // [4 groups][2 halves][span]
   double* const sFar = reinterpret_cast<double*>(smem + 4 * TILE + ((9 * span + 1) / 2 * 2) * 4);  // [4][2]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
@@ -668,26 +687,27 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dq_kernel(RbArgs a)
   double farl = 0., farr = 0.;   // 64 bits: thousands of terms of both signs
   float kept[4] = {0.f, 0.f, 0.f, 0.f};
   bool pending = false;
-  spread_table(a, h, sB, tid, 256);
+  spread_table(a, h, sB, reinterpret_cast<float*>(sK + TILE), TILE / 4, tid);
   for (int x = tid; x < 8 * span; x += 256) sG[x] = 0.f;
   dma_wait();
   __syncthreads();
   const float left = sB[0], right = sB[span - 1];
   // lane's cell for key base 0: its own class (half), or for lanes 0..2 the other half's, 32 keys before
-  const int cls = n32 < 3 ? hi ^ 1 : hi, cell0 = cls * span + 4 * cls + 3 - n32 - (n32 < 3 ? 32 : 0) - p0 + a.md + RB_PAD;
+  const int cls = n32 < 3 ? hi ^ 1 : hi, cell0 = cls * span + 4 * cls + 3 - n32 - (n32 < 3 ? 32 : 0) - p0 + a.mde + RB_PAD;
 
-  for (int t = 0; t < nt; ++t) {
+  auto step = [&](int t, auto parity) {
+    constexpr int buf = decltype(parity)::value;
     const int j0 = t * 64;
     if (t + 1 < nt) {
-      dK.next(lK + ((t + 1) & 1) * TILE, wave);
-      dV.next(lV + ((t + 1) & 1) * TILE, wave);
+      dK.next(lK + (buf ^ 1) * TILE, wave);
+      dV.next(lV + (buf ^ 1) * TILE, wave);
     }
-    const unsigned char* const kt = sK + (t & 1) * TILE;
-    const unsigned char* const vt = sV + (t & 1) * TILE;
+    const unsigned char* const kt = sK + buf * TILE;
+    const unsigned char* const vt = sV + buf * TILE;
     const bool active = j0 < wend;
-    const bool near = active && j0 - (p0 + 31) < a.md && j0 + 63 - p0 > -a.md;
+    const bool near = active && j0 - (p0 + 31) < a.mde && j0 + 63 - p0 > -a.mde;
     const int pw = sq.off + q0;
-    const bool any_near = j0 - (pw + 127) < a.md && j0 + 63 - pw > -a.md;  // of any wave: they share the barrier
+    const bool any_near = j0 - (pw + 127) < a.mde && j0 + 63 - pw > -a.mde;  // of any wave: they share the barrier
     if (!near && pending) {  // the last parts kept have nothing to wait for
 #pragma unroll
       for (int g = 0; g < 4; ++g)
@@ -698,30 +718,52 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dq_kernel(RbArgs a)
     }
     const bool edge = j0 + 64 > sq.klen || (a.causal && j0 + 63 > p0);
     const int lim = (a.causal ? min(sq.klen, p0 + n32 + 1) : sq.klen) - j0 - 4 * hi;
+    const float l2 = near ? lse2 : lse2 - (j0 > p0 ? right : left) * a.c2;  // far: the bias is a constant
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       if (u == 1 && any_near) __syncthreads();
       if (!active) continue;
       f32x16 s, dp = splat16(-delta);
+      // operands in groups ahead of the products that use them, as in rb_fwd_kernel
+      auto scores = [&](auto zero) {
+        constexpr int GK = DP == 128 ? 2 : 4;
+        u32x4 kf[GK], vf[GK];
+#pragma unroll
+        for (int c = 0; c < NK; c += GK) {
+#pragma unroll
+          for (int ks = 0; ks < GK && c + ks < NK; ++ks) {
+            kf[ks] = frag<DP>(kt, 32 * u + n32, c + ks, hi);
+            vf[ks] = frag<DP>(vt, 32 * u + n32, c + ks, hi);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int ks = 0; ks < GK && c + ks < NK; ++ks) {
+            s = E::mma(kf[ks], qf[c + ks], decltype(zero)::value && c + ks == 0 ? splat16(0.f) : s);
+            dp = E::mma(vf[ks], df[c + ks], dp);
+          }
+        }
+      };
       if (near) {
-        const float* const bp = sB + (j0 - p0 - n32 + 4 * hi + 32 * u + a.md + RB_PAD);
+        const float* const bp = sB + (j0 - p0 - n32 + 4 * hi + 32 * u + a.mde + RB_PAD);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = bp[8 * (r >> 2) + (r & 3)];
+        scores(False{});
       } else {
-        s = splat16(j0 > p0 ? right : left);
+        scores(True{});
       }
+      u32x4 kf[2][ND];
 #pragma unroll
-      for (int ks = 0; ks < NK; ++ks) {
-        s = E::mma(frag<DP>(kt, 32 * u + n32, ks, hi), qf[ks], s);
-        dp = E::mma(frag<DP>(vt, 32 * u + n32, ks, hi), df[ks], dp);
-      }
+      for (int kk = 0; kk < (DP == 128 ? 1 : 2); ++kk)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) kf[kk][d] = frag_t<DP>(kt, 32 * u + 16 * kk, d, lane);
+      __builtin_amdgcn_sched_barrier(0);
       if (edge) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (32 * u + 8 * (r >> 2) + (r & 3) >= lim) s[r] = -RB_INF;
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, -lse2)) * dp[r];
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, -l2)) * dp[r];
       if (near) {
         float old[4];
 #pragma unroll
@@ -746,12 +788,21 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dq_kernel(RbArgs a)
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         const u32x4 ds = pack8<E>(s, 8 * kk);
+        if (DP == 128 && kk == 1) {
 #pragma unroll
-        for (int d = 0; d < ND; ++d) dq[d] = E::mma(frag_t<DP>(kt, 32 * u + 16 * kk, d, lane), ds, dq[d]);
+          for (int d = 0; d < ND; ++d) kf[1][d] = frag_t<DP>(kt, 32 * u + 16, d, lane);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dq[d] = E::mma(kf[kk][d], ds, dq[d]);
       }
     }
     dma_wait();
     __syncthreads();
+  };
+  for (int t = 0; t < nt; t += 2) {
+    step(t, Const<0>{});
+    if (t + 1 < nt) step(t + 1, Const<1>{});
   }
   if (pending) {
 #pragma unroll
@@ -797,7 +848,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dq_kernel(RbArgs a)
   for (int n = tid; n < a.nb; n += 256) {
     const int lo = a.bucket_range[2 * n], end = a.bucket_range[2 * n + 1];
     double y = 0.;
-    for (int r = lo; r < end; ++r) y += r == -a.md ? sFar[0] : r == a.md ? sFar[1] : (double)sB[r + a.md + RB_PAD];
+    for (int r = max(lo, -a.mde); r < min(end, a.mde + 1); ++r)
+      y += r == -a.mde ? sFar[0] : r == a.mde ? sFar[1] : (double)sB[r + a.mde + RB_PAD];
     a.part[((int64_t)h * a.nb + n) * nwg + wg] = (float)y;
   }
 }
@@ -814,7 +866,10 @@ DEV void table_sum(const RbArgs& a, int entry, int nwg) {
 }
 
 // dk and dv: 4 waves x 32 keys of one (sequence, key head) against 64-query tiles of every head of its group.
-//   S = Q K^T (+ bias), dP = dO V^T (from -delta), dV^T += dO^T P, dK^T += Q^T dS
+//   S = Q K^T (+ bias), dV^T += dO^T P, dP = dO V^T (from -delta), dK^T += Q^T dS
+// (at a head width of 128 K, V and the sums are 192 registers: one wave a SIMD with 512; two waves spill, 357 us against 95 for the
+// causal 2 x 2047 case).  Where few workgroups would run, the (head, query tile) steps are split over `nsplit`
+// workgroups, whose sums rb_dkv_join_kernel adds in order.
 template <class E, int DP>
 __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -829,7 +884,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
   float* const sB = sL + 256;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const int id = xcd_order(blockIdx.x, a.nblk);
-  const int bh = id / a.ntile, tile = id % a.ntile;
+  const int split = id % a.nsplit, bh = id / a.nsplit / a.ntile, tile = id / a.nsplit % a.ntile;
   const int b = bh / a.Hk, hk = bh % a.Hk, G = a.H / a.Hk;
   const Seq sq = seq_of(a, b);
   const int k0 = tile * 128, j0 = k0 + wave * 32, j = j0 + n32;
@@ -839,17 +894,20 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
   f32x16 dk[ND], dv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dk[d] = dv[d] = splat16(0.f);
-  // causal: the first query that sees key k0 sits at position k0
+  // causal: the first query that sees key k0 sits at position k0.  Steps are numbered head by head.
   const int t0 = a.causal ? max(k0 - sq.off, 0) >> 6 : 0;
-  const int t1 = k0 < sq.klen ? (sq.qlen + 63) >> 6 : 0;
+  const int per = k0 < sq.klen ? max(((sq.qlen + 63) >> 6) - t0, 0) : 0, steps = per * G;
+  const int it0 = (int)((int64_t)steps * split / a.nsplit), it1 = (int)((int64_t)steps * (split + 1) / a.nsplit);
   const unsigned lQ = lds_addr(sQ), lO = lds_addr(sO);
   float lrow = 0.f;
 
-  for (int g = 0; g < G; ++g) {
+  for (int it = it0; it < it1;) {
+    const int g = it / per, ta = t0 + it % per, tb = min(t0 + per, ta + it1 - it);  // one head's run of tiles
+    it += tb - ta;
     const int h = hk * G + g;
     TileDma<DP> dQ, dO;
-    dQ.init(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, t0, sq.qlen, a.D, wave, lane);
-    dO.init(a.dout + b * a.sdo.b + h * a.sdo.h, a.sdo.t, t0, sq.qlen, a.D, wave, lane);
+    dQ.init(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, ta, sq.qlen, a.D, wave, lane);
+    dO.init(a.dout + b * a.sdo.b + h * a.sdo.h, a.sdo.t, ta, sq.qlen, a.D, wave, lane);
     const float* const rl = (wave == 0 ? a.lse2 : a.delta) + ((int64_t)b * a.H + h) * a.tq128;
     auto load = [&](int t, int buf) {
       dQ.next(lQ + buf * TILE, wave);
@@ -860,15 +918,15 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
       if (wave < 2) sL[buf * 128 + wave * 64 + lane] = lrow;
     };
     __syncthreads();  // the head before has been read
-    if (t0 < t1) load(t0, 0);
-    spread_table(a, h, sB, tid, 256);
-    if (t0 < t1) store(0);
+    load(ta, 0);
+    spread_table(a, h, sB, reinterpret_cast<float*>(sQ + TILE), TILE / 4, tid);
+    store(0);
     dma_wait();
     __syncthreads();
-    const float left = sB[0], right = sB[2 * (a.md + RB_PAD)];
-    for (int t = t0; t < t1; ++t) {
-      const int buf = (t - t0) & 1;
-      const bool more = t + 1 < t1;
+    const float left = sB[0], right = sB[2 * (a.mde + RB_PAD)];
+    auto step = [&](int t, auto parity) {
+      constexpr int buf = decltype(parity)::value;
+      const bool more = t + 1 < tb;
       if (more) load(t + 1, buf ^ 1);
       const unsigned char* const qt = sQ + buf * TILE;
       const unsigned char* const ot = sO + buf * TILE;
@@ -878,26 +936,48 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
         const int p0 = sq.off + t * 64 + 32 * u;  // position of the sub-tile's first query
         if (j0 >= sq.klen || (a.causal && j0 > p0 + 31)) continue;
         f32x16 s, dp;
-        if (j0 - (p0 + 31) >= a.md || j0 + 31 - p0 <= -a.md) {
+        if (j0 - (p0 + 31) >= a.mde || j0 + 31 - p0 <= -a.mde) {
           s = splat16(j0 > p0 ? right : left);
         } else {
-          const float* const bp = sB + (j - p0 - 4 * hi + a.md + RB_PAD);
+          const float* const bp = sB + (j - p0 - 4 * hi + a.mde + RB_PAD);
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] = bp[-(8 * (r >> 2) + (r & 3))];
         }
-        float ls[16];
+        auto product = [&](const unsigned char* tile, const u32x4 (&f)[NK], f32x16& x) {  // x += rows of the tile . f
+          constexpr int GK = 4;
+          u32x4 af[GK];
+#pragma unroll
+          for (int c = 0; c < NK; c += GK) {
+#pragma unroll
+            for (int ks = 0; ks < GK && c + ks < NK; ++ks) af[ks] = frag<DP>(tile, 32 * u + n32, c + ks, hi);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks < GK && c + ks < NK; ++ks) x = E::mma(af[ks], f[c + ks], x);
+          }
+        };
+        auto outer = [&](const unsigned char* tile, const f32x16& x, f32x16 (&sum)[ND]) {  // sum += tile^T . x, x rounded here
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk) {
+            u32x4 af[ND];
+#pragma unroll
+            for (int d = 0; d < ND; ++d) af[d] = frag_t<DP>(tile, 32 * u + 16 * kk, d, lane);
+            const u32x4 xb = pack8<E>(x, 8 * kk);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) sum[d] = E::mma(af[d], xb, sum[d]);
+          }
+        };
+        product(qt, kf, s);
+        f32x4 ls[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ls[q] = *reinterpret_cast<const f32x4*>(lt + 32 * u + 8 * q + 4 * hi);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(lt + 32 * u + 8 * q + 4 * hi);
           const f32x4 y = *reinterpret_cast<const f32x4*>(lt + 64 + 32 * u + 8 * q + 4 * hi);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) ls[4 * q + r] = x[r], dp[4 * q + r] = y[r];
+          for (int r = 0; r < 4; ++r) dp[4 * q + r] = y[r];
         }
-#pragma unroll
-        for (int ks = 0; ks < NK; ++ks) {
-          s = E::mma(frag<DP>(qt, 32 * u + n32, ks, hi), kf[ks], s);
-          dp = E::mma(frag<DP>(ot, 32 * u + n32, ks, hi), vf[ks], dp);
-        }
+        product(ot, vf, dp);
         if (a.causal && j0 + 31 > p0) {
           const int lim = j - p0 - 4 * hi;  // queries before it do not see the key
 #pragma unroll
@@ -906,26 +986,37 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, -ls[r]));
+          s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, -ls[r >> 2][r & 3]));
           dp[r] *= s[r];
         }
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          const u32x4 pb = pack8<E>(s, 8 * kk), db = pack8<E>(dp, 8 * kk);
-#pragma unroll
-          for (int d = 0; d < ND; ++d) {
-            dv[d] = E::mma(frag_t<DP>(ot, 32 * u + 16 * kk, d, lane), pb, dv[d]);
-            dk[d] = E::mma(frag_t<DP>(qt, 32 * u + 16 * kk, d, lane), db, dk[d]);
-          }
-        }
+        outer(ot, s, dv);
+        outer(qt, dp, dk);
       }
       if (more) store(buf ^ 1);
       dma_wait();
       __syncthreads();
+    };
+    for (int t = ta; t < tb; t += 2) {
+      step(t, Const<0>{});
+      if (t + 1 < tb) step(t + 1, Const<1>{});
     }
   }
   table_sum(a, blockIdx.x * 4 + wave, a.B * a.nqtile);  // each wave one entry of the table's gradient, from the dq kernel's shares
   if (j >= a.Tk) return;
+  if (a.nsplit > 1) {  // sums in f32: [split][dk | dv][sequence, key head, key][DP]
+    const int64_t rows = (int64_t)a.B * a.Hk * a.Tk, row = ((int64_t)b * a.Hk + hk) * a.Tk + j;
+    float* const pk = a.part2 + ((int64_t)split * 2 * rows + row) * DP;
+    float* const pv = pk + rows * DP;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = 32 * d + 8 * g + 4 * hi;
+        *reinterpret_cast<f32x4*>(pk + c) = f32x4{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]};
+        *reinterpret_cast<f32x4*>(pv + c) = f32x4{dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]};
+      }
+    return;
+  }
   const bool in = j < sq.klen;  // rows behind the sequence get zeros
   uint16_t* const kp = a.dk + b * a.sdk.b + (int64_t)j * a.sdk.t + hk * a.sdk.h;
   uint16_t* const vp = a.dv + b * a.sdv.b + (int64_t)j * a.sdv.t + hk * a.sdv.h;
@@ -941,6 +1032,24 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
       store4<E>(kp + c, x[0], x[1], x[2], x[3]);
       store4<E>(vp + c, x[4], x[5], x[6], x[7]);
     }
+}
+
+// dk and dv from the splits' sums, in order; a thread has 4 elements of one row of one of the two
+template <class E, int DP>
+__global__ __launch_bounds__(256) void rb_dkv_join_kernel(RbArgs a) {
+  const int64_t rows = (int64_t)a.B * a.Hk * a.Tk, x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t r2 = x / (DP / 4);
+  const int c = (int)(x % (DP / 4)) * 4;
+  if (r2 >= 2 * rows || c >= a.D) return;
+  const int64_t row = r2 % rows, bh = row / a.Tk;
+  const int j = (int)(row % a.Tk), b = (int)(bh / a.Hk), hk = (int)(bh % a.Hk);
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.nsplit; ++s) y += *reinterpret_cast<const f32x4*>(a.part2 + ((int64_t)s * 2 * rows + r2) * DP + c);
+  const bool key = r2 < rows;
+  const Strides st = key ? a.sdk : a.sdv;
+  if (key) y *= a.scale;
+  if (j >= seq_of(a, b).klen) y = f32x4{0.f, 0.f, 0.f, 0.f};
+  store4<E>((key ? a.dk : a.dv) + b * st.b + (int64_t)j * st.t + hk * st.h + c, y[0], y[1], y[2], y[3]);
 }
 
 // =============================================================================================== host side
@@ -968,6 +1077,14 @@ int check_args(const csship_relbias* p) {
   return CSSHIP_OK;
 }
 
+// the largest distance whose table entry a call can need: with one offset for all sequences, no pair is further apart than this
+int reach(const csship_relbias* p) {
+  if (p->offsets != nullptr) return p->max_distance;
+  const int off = p->offset < -RB_MAX_POS ? -RB_MAX_POS : p->offset > RB_MAX_POS ? RB_MAX_POS : p->offset;
+  const int back = p->Tq - 1 + off, front = p->Tk - 1 - off, far = (back > front ? back : front) + 1;
+  return far < 1 ? 1 : far < p->max_distance ? far : p->max_distance;
+}
+
 RbArgs to_args(const csship_relbias* p) {
   RbArgs a{};
   a.q = p->q; a.k = p->k; a.v = p->v;
@@ -975,7 +1092,7 @@ RbArgs to_args(const csship_relbias* p) {
   a.table = p->table; a.bucket_of = p->bucket_of; a.bucket_range = p->bucket_range;
   a.k_lens = p->k_lens; a.q_lens = p->q_lens; a.offsets = p->offsets;
   a.B = p->B; a.Tq = p->Tq; a.Tk = p->Tk; a.H = p->H; a.Hk = p->Hk; a.D = p->D;
-  a.nb = p->n_buckets; a.md = p->max_distance; a.causal = p->causal != 0; a.offset = p->offset;
+  a.nb = p->n_buckets; a.md = p->max_distance; a.mde = reach(p); a.causal = p->causal != 0; a.offset = p->offset;
   a.scale = p->scale; a.inv_scale = 1.f / p->scale; a.c2 = p->scale * RB_LOG2E;
   return a;
 }
@@ -1024,20 +1141,32 @@ int launch_fwd(RbArgs a, const csship_relbias* p, hipStream_t s) {
   a.ntile = (a.Tq + 127) / 128;
   a.nblk = a.B * a.H * a.ntile;
   if (a.nblk == 0) return CSSHIP_OK;
-  return launch(rb_fwd_kernel<E, DP>, a.nblk, fwd_lds(DP, a.md), a, s);
+  return launch(rb_fwd_kernel<E, DP>, a.nblk, fwd_lds(DP, a.mde), a, s);
+}
+
+// Workgroups of the dk / dv kernel take 128 keys of a sequence and key head; where those leave most of the chip idle, each one's
+// steps (64 queries of one head) are split, at most 8 ways and not below 8 steps.
+int dkv_splits(const csship_relbias* p) {
+  const int64_t wgs = (int64_t)p->B * p->Hk * ((p->Tk + 127) / 128), steps = (int64_t)(p->H / p->Hk) * ((p->Tq + 63) / 64);
+  if (wgs == 0) return 1;
+  const int64_t want = 512 / wgs, most = steps / 8 < 8 ? steps / 8 : 8;
+  return (int)(want < 1 || most < 1 ? 1 : want < most ? want : most);
 }
 
 template <class E, int DP>
-int launch_bwd(RbArgs a, hipStream_t s) {
+int launch_bwd(RbArgs a, const csship_relbias* p, hipStream_t s) {
   a.ntile = a.nqtile = (a.Tq + 127) / 128;
   a.tq128 = a.ntile * 128;
   a.nblk = a.B * a.H * a.ntile;
   if (a.nblk > 0)
-    if (const int rc = launch(rb_dq_kernel<E, DP>, a.nblk, dq_lds(DP, a.md), a, s)) return rc;
+    if (const int rc = launch(rb_dq_kernel<E, DP>, a.nblk, dq_lds(DP, a.mde), a, s)) return rc;
   a.ntile = (a.Tk + 127) / 128;
-  a.nblk = a.B * a.Hk * a.ntile;
+  a.nsplit = dkv_splits(p);
+  a.nblk = a.B * a.Hk * a.ntile * a.nsplit;
   const int64_t entries = ((int64_t)a.nb * a.H + 3) / 4;
-  return launch(rb_dkv_kernel<E, DP>, a.nblk > entries ? a.nblk : entries, dkv_lds(DP, a.md), a, s);
+  if (const int rc = launch(rb_dkv_kernel<E, DP>, a.nblk > entries ? a.nblk : entries, dkv_lds(DP, a.mde), a, s)) return rc;
+  if (a.nsplit == 1) return CSSHIP_OK;
+  return launch(rb_dkv_join_kernel<E, DP>, ((int64_t)2 * a.B * a.Hk * a.Tk * (DP / 4) + 255) / 256, 0, a, s);
 }
 
 template <class E>
@@ -1045,11 +1174,14 @@ int fwd_by_width(const RbArgs& a, const csship_relbias* p, hipStream_t s) {
   return a.D <= 32 ? launch_fwd<E, 32>(a, p, s) : a.D <= 64 ? launch_fwd<E, 64>(a, p, s) : launch_fwd<E, 128>(a, p, s);
 }
 template <class E>
-int bwd_by_width(const RbArgs& a, hipStream_t s) {
-  return a.D <= 32 ? launch_bwd<E, 32>(a, s) : a.D <= 64 ? launch_bwd<E, 64>(a, s) : launch_bwd<E, 128>(a, s);
+int bwd_by_width(const RbArgs& a, const csship_relbias* p, hipStream_t s) {
+  return a.D <= 32 ? launch_bwd<E, 32>(a, p, s) : a.D <= 64 ? launch_bwd<E, 64>(a, p, s) : launch_bwd<E, 128>(a, p, s);
 }
 
 int64_t row_words(const csship_relbias* p) { return (int64_t)p->B * p->H * ((p->Tq + 127) / 128 * 128); }
+
+// the table gradient's shares: one number per workgroup of the dq kernel and bucket, in whole 16 bytes
+int64_t part_words(const csship_relbias* p) { return ((int64_t)p->B * p->H * ((p->Tq + 127) / 128) * p->n_buckets + 3) / 4 * 4; }
 
 }  // namespace
 
@@ -1081,8 +1213,9 @@ int csship_relbias_fwd(const csship_relbias* p, uint16_t* out, const int64_t* ou
 
 size_t csship_relbias_bwd_workspace(const csship_relbias* p) {
   if (check_args(p) != CSSHIP_OK) return 0;
-  const int64_t wgs = (int64_t)p->B * p->H * ((p->Tq + 127) / 128);
-  return (size_t)(2 * row_words(p) + wgs * p->n_buckets) * 4 + 16;
+  const int splits = dkv_splits(p);
+  const int64_t sums = splits == 1 ? 0 : (int64_t)splits * 2 * p->B * p->Hk * p->Tk * width_of(p->D);
+  return (size_t)(2 * row_words(p) + part_words(p) + sums) * 4 + 16;
 }
 
 int csship_relbias_bwd(const csship_relbias* p, const uint16_t* out, const int64_t* out_stride, const float* lse, const uint16_t* dout,
@@ -1111,7 +1244,8 @@ int csship_relbias_bwd(const csship_relbias* p, const uint16_t* out, const int64
   a.delta = static_cast<float*>(workspace);
   a.lse2 = a.delta + row_words(p);
   a.part = a.lse2 + row_words(p);
-  return p->dtype == CSSHIP_RELBIAS_BF16 ? bwd_by_width<ElemBf>(a, as_stream(stream)) : bwd_by_width<ElemHf>(a, as_stream(stream));
+  a.part2 = a.part + part_words(p);
+  return p->dtype == CSSHIP_RELBIAS_BF16 ? bwd_by_width<ElemBf>(a, p, as_stream(stream)) : bwd_by_width<ElemHf>(a, p, as_stream(stream));
 }
 
 }  // extern "C"
