@@ -140,6 +140,12 @@ DEV float half_sum(float x) {
   return __uint_as_float(a0) + __uint_as_float(a1);
 }
 
+DEV double wave_total(double x) {
+#pragma unroll
+  for (int w = 1; w < 64; w <<= 1) x += __shfl_xor(x, w);
+  return x;
+}
+
 // ---- 64-row tiles of a [T, heads, D] tensor, memory -> LDS without passing registers (buffer_load_dwordx4 ... lds): one
 // instruction of a wave fills 1 KB in lane order, so the swizzle is applied to the address each lane fetches.  Rows at or behind
 // `rows` and pieces at or behind D / 8 lie outside the descriptor: zeros.  Written as inline assembly because the compiler, which
@@ -178,14 +184,18 @@ struct TileDma {
 DEV void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 DEV unsigned lds_addr(const void* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p; }
 
-// one lane's operand fragments of row `row` (piece 2 ks + hi), zeros where the row does not count
+// a lane's operand fragments (pieces 2 ks + hi) of row first + (lane & 31), zeros where the row does not count (first + .. >= rows).
+// Descriptor loads: no branch around a load, all of them in flight together.
 template <int DP>
-DEV void row_frags(const uint16_t* base, int64_t st, int row, bool valid, int D, int hi, u32x4 (&f)[DP / 16]) {
+DEV void row_frags(const uint16_t* base, int64_t st, int first, int rows, int D, int lane, u32x4 (&f)[DP / 16]) {
+  const __amdgpu_buffer_rsrc_t rs =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base + (int64_t)first * st), 0, 0x7ffffff0, 0x00020000);
+  const int n = lane & 31, hi = lane >> 5;
 #pragma unroll
   for (int ks = 0; ks < DP / 16; ++ks) {
     const int c = 2 * ks + hi;
-    f[ks] = u32x4{0, 0, 0, 0};
-    if (valid && c * 8 < D) f[ks] = *reinterpret_cast<const u32x4*>(base + (int64_t)row * st + c * 8);
+    f[ks] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                          rs, first + n < rows && c * 8 < D ? (int)((unsigned)n * (unsigned)st * 2u + c * 16u) : -16, 0, 0));
   }
 }
 
@@ -270,7 +280,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
   u32x4 qf[NK];
   f32x16 o[ND];
   float m = -RB_INF, l = 0.f;
-  row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, i, i < sq.qlen, a.D, hi, qf);
+  row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, q0 + wave * 32, sq.qlen, a.D, lane, qf);
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = splat16(0.f);
   spread_table(a, h, sB, reinterpret_cast<float*>(sK + TILE), TILE / 4, tid);
@@ -282,10 +292,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
   auto step = [&](int t, auto parity) {
     constexpr int buf = decltype(parity)::value;
     const int j0 = t * 64;
-    if (t + 1 < nt) {
+    // the next tile's transfer: requested behind the first products, whose results the wave waits for anyway
+    auto transfer = [&] {
+      if (t + 1 >= nt) return;
       dk.next(lK + (buf ^ 1) * TILE, wave);
       dv.next(lV + (buf ^ 1) * TILE, wave);
-    }
+    };
     if (j0 < wend) {
       const unsigned char* const kt = sK + buf * TILE;
       const unsigned char* const vt = sV + buf * TILE;
@@ -321,6 +333,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
           for (int r = 0; r < 16; ++r) s[u][r] = bp[32 * u + 8 * (r >> 2) + (r & 3)];
         scores(False{});
       }
+      transfer();
       u32x4 vf[2][ND];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
@@ -380,6 +393,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] = E::mma(vg[kk][d], pb[2 + kk], o[d]);
+    } else {
+      transfer();
     }
     dma_wait();
     __syncthreads();
@@ -419,7 +434,12 @@ __global__ __launch_bounds__(256, 2) void rb_few_kernel(RbArgs a) {
   const uint16_t* const vp = a.v + b * a.sv.b + hk * a.sv.h;
 
   u32x4 qf[NK], kf[NK], vr[NV];
-  row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, i, valid, a.D, hi, qf);
+#pragma unroll
+  for (int ks = 0; ks < NK; ++ks) {
+    const int c = 2 * ks + hi;
+    qf[ks] = u32x4{0, 0, 0, 0};
+    if (valid && c * 8 < a.D) qf[ks] = *reinterpret_cast<const u32x4*>(a.q + b * a.sq.b + (int64_t)i * a.sq.t + h * a.sq.h + c * 8);
+  }
   const int hc = min(h, a.H - 1);
   const float left = bias_entry(a, -a.md, hc), right = bias_entry(a, a.md, hc);
   auto load = [&](int t) {
@@ -641,7 +661,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   float* const sB = reinterpret_cast<float*>(smem + 4 * TILE);
   const int span = 2 * (a.mde + RB_PAD) + 1;
   float* const sG = sB + span;                                      // [4 groups][2 halves][span]
-  double* const sFar = reinterpret_cast<double*>(smem + 4 * TILE + ((9 * span + 1) / 2 * 2) * 4);  // [4][2]
+  double* const sFar = reinterpret_cast<double*>(smem + 4 * TILE + ((9 * span + 1) / 2 * 2) * 4);  // [4][2], [4]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const int id = xcd_order(blockIdx.x, a.nblk);
   const int bh = id / a.ntile, tile = a.ntile - 1 - id % a.ntile;
@@ -664,14 +684,15 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
     dV.next(lV, wave);
   }
   u32x4 qf[NK], df[NK];
-  row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, i, i < sq.qlen, a.D, hi, qf);
-  row_frags<DP>(a.dout + b * a.sdo.b + h * a.sdo.h, a.sdo.t, i, i < sq.qlen, a.D, hi, df);
+  row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, q0 + wave * 32, sq.qlen, a.D, lane, qf);
+  row_frags<DP>(a.dout + b * a.sdo.b + h * a.sdo.h, a.sdo.t, q0 + wave * 32, sq.qlen, a.D, lane, df);
   float delta = 0.f, lse2 = RB_INF;
   {
     u32x4 of[NK];
-    row_frags<DP>(a.o + b * a.so.b + h * a.so.h, a.so.t, i, i < sq.qlen, a.D, hi, of);
-    const int64_t at = ((int64_t)b * a.H + h) * a.Tq + i;
-    const float x = i < sq.qlen ? a.lse_in[at] : -RB_INF;
+    row_frags<DP>(a.o + b * a.so.b + h * a.so.h, a.so.t, q0 + wave * 32, sq.qlen, a.D, lane, of);
+    const float given = a.lse_in[((int64_t)b * a.H + h) * a.Tq + min(i, a.Tq - 1)];
+    for (int x = tid; x < 8 * span; x += 256) sG[x] = 0.f;
+    const float x = i < sq.qlen ? given : -RB_INF;
 #pragma unroll
     for (int ks = 0; ks < NK; ++ks)
 #pragma unroll
@@ -688,7 +709,6 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   float kept[4] = {0.f, 0.f, 0.f, 0.f};
   bool pending = false;
   spread_table(a, h, sB, reinterpret_cast<float*>(sK + TILE), TILE / 4, tid);
-  for (int x = tid; x < 8 * span; x += 256) sG[x] = 0.f;
   dma_wait();
   __syncthreads();
   const float left = sB[0], right = sB[span - 1];
@@ -698,10 +718,12 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   auto step = [&](int t, auto parity) {
     constexpr int buf = decltype(parity)::value;
     const int j0 = t * 64;
-    if (t + 1 < nt) {
+    auto transfer = [&] {  // the next tile's, behind the first products as in rb_fwd_kernel
+      if (t + 1 >= nt) return;
       dK.next(lK + (buf ^ 1) * TILE, wave);
       dV.next(lV + (buf ^ 1) * TILE, wave);
-    }
+    };
+    if (!(j0 < wend)) transfer();
     const unsigned char* const kt = sK + buf * TILE;
     const unsigned char* const vt = sV + buf * TILE;
     const bool active = j0 < wend;
@@ -751,9 +773,10 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
       } else {
         scores(True{});
       }
+      if (u == 0) transfer();
       u32x4 kf[2][ND];
 #pragma unroll
-      for (int kk = 0; kk < (DP == 128 ? 1 : 2); ++kk)
+      for (int kk = 0; kk < (DP == 128 ? 0 : 2); ++kk)
 #pragma unroll
         for (int d = 0; d < ND; ++d) kf[kk][d] = frag_t<DP>(kt, 32 * u + 16 * kk, d, lane);
       __builtin_amdgcn_sched_barrier(0);
@@ -788,10 +811,9 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         const u32x4 ds = pack8<E>(s, 8 * kk);
-        if (DP == 128 && kk == 1) {
+        if (DP == 128) {  // (no registers to hold them across the exponentials)
 #pragma unroll
-          for (int d = 0; d < ND; ++d) kf[1][d] = frag_t<DP>(kt, 32 * u + 16, d, lane);
-          __builtin_amdgcn_sched_barrier(0);
+          for (int d = 0; d < ND; ++d) kf[kk][d] = frag_t<DP>(kt, 32 * u + 16 * kk, d, lane);
         }
 #pragma unroll
         for (int d = 0; d < ND; ++d) dq[d] = E::mma(kf[kk][d], ds, dq[d]);
@@ -821,35 +843,50 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
           store4<E>(op + c, dq[d][4 * g] * a.scale, dq[d][4 * g + 1] * a.scale, dq[d][4 * g + 2] * a.scale, dq[d][4 * g + 3] * a.scale);
       }
   }
-  // the workgroup's share of the table's gradient: by distance (arrays in order), then by bucket
-#pragma unroll
-  for (int w = 1; w < 64; w <<= 1) {
-    farl += __shfl_xor(farl, w);
-    farr += __shfl_xor(farr, w);
-  }
+  // The workgroup's share of the table's gradient.  A bucket's distances are contiguous: running sums over the distances in 64
+  // bits, and a bucket is the difference of two (one thread per bucket adding up its distances took 4 us).
+  const int nwg = a.B * a.ntile, wg = b * a.ntile + tile;
+  int lo = 0, end = 0;
+  if (tid < a.nb) lo = a.bucket_range[2 * tid], end = a.bucket_range[2 * tid + 1];
+  farl = wave_total(farl);
+  farr = wave_total(farr);
   if (lane == 0) sFar[2 * wave] = farl, sFar[2 * wave + 1] = farr;
   __syncthreads();
-  for (int x = tid; x < span; x += 256) {
+  const int each = (span + 255) >> 8, first = tid * each;
+  double mine = 0.;
+  for (int x = first; x < min(first + each, span); ++x) {
     float y = 0.f;
 #pragma unroll
     for (int c = 0; c < 8; ++c) y += sG[c * span + x];
     sB[x] = y;
+    mine += (double)y;
   }
-  __syncthreads();
-  if (wave < 2) {  // the two ends hold everything beyond them
-    double y = 0.;
-    for (int x = lane; x <= RB_PAD; x += 64) y += (double)sB[wave == 0 ? x : span - 1 - x];
+  double upto = mine;  // inclusive over the wave, then over the workgroup
 #pragma unroll
-    for (int w = 1; w < 64; w <<= 1) y += __shfl_xor(y, w);
-    if (lane == 0) sFar[wave] = y + ((sFar[wave] + sFar[2 + wave]) + (sFar[4 + wave] + sFar[6 + wave]));
+  for (int w = 1; w < 64; w <<= 1) {
+    const double y = __shfl_up(upto, w);
+    if (lane >= w) upto += y;
+  }
+  if (lane == 63) sFar[8 + wave] = upto;
+  __syncthreads();  // sG has been read: the running sums take its place
+  double* const run = reinterpret_cast<double*>(smem + 4 * TILE + (span + 1) / 2 * 8);  // [span + 1]
+  upto -= mine;
+  for (int w = 0; w < wave; ++w) upto += sFar[8 + w];
+  for (int x = first; x < min(first + each, span); ++x) {
+    run[x] = upto;
+    upto += (double)sB[x];
+    if (x == span - 1) run[span] = upto;
   }
   __syncthreads();
-  const int nwg = a.B * a.ntile, wg = b * a.ntile + tile;
+  const double lefts = (sFar[0] + sFar[2]) + (sFar[4] + sFar[6]), rights = (sFar[1] + sFar[3]) + (sFar[5] + sFar[7]);
   for (int n = tid; n < a.nb; n += 256) {
-    const int lo = a.bucket_range[2 * n], end = a.bucket_range[2 * n + 1];
+    if (n != tid) lo = a.bucket_range[2 * n], end = a.bucket_range[2 * n + 1];
     double y = 0.;
-    for (int r = max(lo, -a.mde); r < min(end, a.mde + 1); ++r)
-      y += r == -a.mde ? sFar[0] : r == a.mde ? sFar[1] : (double)sB[r + a.mde + RB_PAD];
+    if (lo < end && end > -a.mde && lo <= a.mde) {  // the ends hold everything beyond them
+      y = run[end > a.mde ? span : end + a.mde + RB_PAD] - run[lo <= -a.mde ? 0 : lo + a.mde + RB_PAD];
+      if (lo <= -a.mde) y += lefts;
+      if (end > a.mde) y += rights;
+    }
     a.part[((int64_t)h * a.nb + n) * nwg + wg] = (float)y;
   }
 }
@@ -860,8 +897,7 @@ DEV void table_sum(const RbArgs& a, int entry, int nwg) {
   const int lane = threadIdx.x & 63, h = entry / a.nb, n = entry % a.nb;
   double s = 0.;
   for (int x = lane; x < nwg; x += 64) s += (double)a.part[(int64_t)entry * nwg + x];
-#pragma unroll
-  for (int w = 1; w < 64; w <<= 1) s += __shfl_xor(s, w);
+  s = wave_total(s);
   if (lane == 0) a.dtable[n * a.H + h] = (float)s;
 }
 
@@ -889,8 +925,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
   const Seq sq = seq_of(a, b);
   const int k0 = tile * 128, j0 = k0 + wave * 32, j = j0 + n32;
   u32x4 kf[NK], vf[NK];
-  row_frags<DP>(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, j, j < sq.klen, a.D, hi, kf);
-  row_frags<DP>(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, j, j < sq.klen, a.D, hi, vf);
+  row_frags<DP>(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, j0, sq.klen, a.D, lane, kf);
+  row_frags<DP>(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, j0, sq.klen, a.D, lane, vf);
   f32x16 dk[ND], dv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dk[d] = dv[d] = splat16(0.f);
@@ -1098,7 +1134,7 @@ RbArgs to_args(const csship_relbias* p) {
 }
 
 size_t fwd_lds(int DP, int md) { return (size_t)4 * 64 * 2 * DP + (2 * (md + RB_PAD) + 1) * 4; }
-size_t dq_lds(int DP, int md) { return (size_t)4 * 64 * 2 * DP + (size_t)(9 * (2 * (md + RB_PAD) + 1) + 1) / 2 * 2 * 4 + 64; }
+size_t dq_lds(int DP, int md) { return (size_t)4 * 64 * 2 * DP + (size_t)(9 * (2 * (md + RB_PAD) + 1) + 1) / 2 * 2 * 4 + 96; }
 size_t dkv_lds(int DP, int md) { return fwd_lds(DP, md) + 1024; }
 
 // launches with more than 64 KB of LDS have to be allowed, per device: asked for at each such launch
