@@ -408,40 +408,38 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
 
 // ------------------------------------------------------------------------------------ forward, few query rows
 // Rows = (query, head of the group) of one (sequence, key head), 32 to a workgroup: a head's group shares the K and V it reads.
-// Nothing is reused across waves, so each of the 4 waves streams its own 32-key tiles (every fourth of the workgroup's), K straight
+// Nothing is reused across waves, so each of the NW waves streams its own 32-key tiles (every NW-th of the workgroup's), K straight
 // into operand registers, V through a wave's own LDS tile for the transposing reads, the next tile's loads in flight; the waves'
 // running softmax states are joined in LDS.  Bound by the bytes of K and V.  Where few workgroups would run, the keys are split
 // over `nsplit` of them: states go to the workspace and rb_join_kernel joins them in order.
-template <class E, int DP>
-__global__ __launch_bounds__(256, 2) void rb_few_kernel(RbArgs a) {
+constexpr int RB_FEW_TABLE = 4096;  // floats of LDS for the group's tables by distance; wider ones are gathered from memory
+template <int DP, int NW>
+constexpr int few_area() {  // bytes: the waves' V tiles, later their O rows [NW][32][DP + 4] and (reference, sum) [NW][2][32]
+  return NW * 32 * (DP + 4) * 4 + NW * 256;
+}
+template <class E, int DP, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void rb_few_kernel(RbArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  constexpr int P = 2 * DP, NK = DP / 16, ND = DP / 32, CPR = DP / 8, RPI = 64 / CPR, NV = 32 / RPI;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, n32 = lane & 31;
+  constexpr int P = 2 * DP, NK = DP / 16, ND = DP / 32, CPR = DP / 8, RPI = 64 / CPR, NV = 32 / RPI, NT = 64 * NW;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   unsigned char* const sV = smem + wave * 32 * P;
+  float* const sT = reinterpret_cast<float*>(smem + few_area<DP, NW>());
   const int G = a.H / a.Hk, R = a.Tq * G;
   const int id = xcd_order(blockIdx.x, a.nblk);
   const int split = id % a.nsplit, rb = id / a.nsplit % a.ntile, bk = id / a.nsplit / a.ntile;
   const int b = bk / a.Hk, hk = bk % a.Hk;
   const Seq sq = seq_of(a, b);
-  const int row = rb * 32 + n32, i = row / G, h = hk * G + row % G;
+  const int row = rb * 32 + n32, i = row / G, g = row - i * G, h = hk * G + g;
   const bool valid = row < R && i < sq.qlen;
   const int p = sq.off + i, i_last = min((rb * 32 + 31) / G, sq.qlen - 1);
   int kend = rb * 32 / G < sq.qlen ? sq.klen : 0;
   if (a.causal) kend = min(kend, sq.off + i_last + 1);
   const int ntile = kend > 0 ? (kend + 31) >> 5 : 0, per = (ntile + a.nsplit - 1) / a.nsplit;
-  const int t1 = min(ntile, (split + 1) * per);
+  const int t0 = split * per, t1 = min(ntile, t0 + per);
   const uint16_t* const kp = a.k + b * a.sk.b + hk * a.sk.h;
   const uint16_t* const vp = a.v + b * a.sv.b + hk * a.sv.h;
 
   u32x4 qf[NK], kf[NK], vr[NV];
-#pragma unroll
-  for (int ks = 0; ks < NK; ++ks) {
-    const int c = 2 * ks + hi;
-    qf[ks] = u32x4{0, 0, 0, 0};
-    if (valid && c * 8 < a.D) qf[ks] = *reinterpret_cast<const u32x4*>(a.q + b * a.sq.b + (int64_t)i * a.sq.t + h * a.sq.h + c * 8);
-  }
-  const int hc = min(h, a.H - 1);
-  const float left = bias_entry(a, -a.md, hc), right = bias_entry(a, a.md, hc);
   auto load = [&](int t) {
     const int j0 = t * 32, left_rows = sq.klen - j0;
     const __amdgpu_buffer_rsrc_t rk =
@@ -461,28 +459,48 @@ __global__ __launch_bounds__(256, 2) void rb_few_kernel(RbArgs a) {
                                             rv, r < left_rows && c * 8 < a.D ? (int)((unsigned)r * (unsigned)a.sv.t * 2u + c * 16) : -16, 0, 0));
     }
   };
+  int t = t0 + wave;
+  if (t < t1) load(t);
+  const uint16_t* const qp = a.q + b * a.sq.b + (int64_t)(valid ? i : 0) * a.sq.t + (valid ? h : hk * G) * a.sq.h;
+#pragma unroll
+  for (int ks = 0; ks < NK; ++ks) {  // (a row that does not count reads row 0 and drops it)
+    const int c = 2 * ks + hi;
+    qf[ks] = u32x4{0, 0, 0, 0};
+    if (a.Tq > 0 && c * 8 < a.D) qf[ks] = *reinterpret_cast<const u32x4*>(qp + c * 8);
+    if (!valid) qf[ks] = u32x4{0, 0, 0, 0};
+  }
+  const int hc = hk * G + min(g, G - 1);
+  const float left = bias_entry(a, -a.mde, hc), right = bias_entry(a, a.mde, hc);
+  const int p_lo = sq.off + rb * 32 / G, p_hi = sq.off + (rb * 32 + 31) / G;  // positions of the workgroup's rows
+  // the group's tables by distance, if any tile of the workgroup's needs them
+  const int wide = 2 * a.mde + 1;
+  const bool staged = G * wide <= RB_FEW_TABLE;
+  if (staged && t0 < t1 && t0 * 32 - p_hi < a.mde && t1 * 32 - 1 - p_lo > -a.mde) {
+    for (int x = tid; x < G * wide; x += NT) sT[x] = bias_entry(a, x % wide - a.mde, hk * G + x / wide);
+    __syncthreads();
+  }
+  const float* const tp = sT + min(g, G - 1) * wide + a.mde;
   f32x16 o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = splat16(0.f);
   float m = -RB_INF, l = 0.f;
-  int t = __builtin_amdgcn_readfirstlane(split * per + wave);
-  if (t < t1) load(t);
-  const int p_lo = sq.off + rb * 32 / G, p_hi = sq.off + (rb * 32 + 31) / G;  // positions of the workgroup's rows
-  for (; t < t1; t += 4) {
+  for (; t < t1; t += NW) {
     const int j0 = t * 32;
     f32x16 s;
-    if (j0 - p_hi >= a.md || j0 + 31 - p_lo <= -a.md) {
+    if (j0 - p_hi >= a.mde || j0 + 31 - p_lo <= -a.mde) {
       s = splat16(j0 > p_lo ? right : left);
-    } else {  // a few tiles of a long context: gathered from the cached table
+    } else {
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        s[r] = bias_entry(a, min(max(j0 + 8 * (r >> 2) + 4 * hi + (r & 3) - p, -a.md), a.md), hc);
+      for (int r = 0; r < 16; ++r) {
+        const int dist = min(max(j0 + 8 * (r >> 2) + 4 * hi + (r & 3) - p, -a.mde), a.mde);
+        s[r] = staged ? tp[dist] : bias_entry(a, dist, hc);
+      }
     }
 #pragma unroll
     for (int ks = 0; ks < NK; ++ks) s = E::mma(kf[ks], qf[ks], s);
 #pragma unroll
     for (int n = 0; n < NV; ++n) *reinterpret_cast<u32x4*>(sV + tile_at<DP>(n * RPI + lane / CPR, lane % CPR)) = vr[n];
-    if (t + 4 < t1) load(t + 4);
+    if (t + NW < t1) load(t + NW);
     if (j0 + 32 > sq.klen || (a.causal && j0 + 31 > p_lo)) {
       const int lim = (a.causal ? min(sq.klen, p + 1) : sq.klen) - j0 - 4 * hi;
 #pragma unroll
@@ -520,65 +538,51 @@ __global__ __launch_bounds__(256, 2) void rb_few_kernel(RbArgs a) {
     __builtin_amdgcn_wave_barrier();
   }
 
-  // join the 4 waves: reference, sum, rows of O [32][DP + 4] f32 (the padding spreads a column's 32 rows over the banks)
+  // join the waves: rows of O [NW][32][DP + 4] f32 (the padding spreads a column's 32 rows over the banks), references, sums
   l = half_sum(l);
   float* const sO = reinterpret_cast<float*>(smem);
-  float* const sM = sO + 32 * (DP + 4);  // [4][2][32]
-  __syncthreads();                       // the V tiles are read
-  if (hi == 0) sM[wave * 64 + n32] = m, sM[wave * 64 + 32 + n32] = l;
-  __syncthreads();
-  float mall = sM[n32], lall = 0.f;
+  float* const sM = sO + NW * 32 * (DP + 4);  // [NW][2][32]
+  __syncthreads();                            // the V tiles are read
+  if (hi == 0) sM[wave * 64 + n32] = m, sM[wave * 64 + 32 + n32] = valid ? l : 0.f;
 #pragma unroll
-  for (int w = 1; w < 4; ++w) mall = fmaxf(mall, sM[w * 64 + n32]);
+  for (int d = 0; d < ND; ++d)
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float mw = sM[w * 64 + n32];
-    lall += mw == -RB_INF ? 0.f : sM[w * 64 + 32 + n32] * __builtin_amdgcn_exp2f((mw - mall) * a.c2);
-  }
-  const float mine = m == -RB_INF ? 0.f : __builtin_amdgcn_exp2f((m - mall) * a.c2);
-  for (int w = 0; w < 4; ++w) {  // in order
-    if (wave == w) {
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          f32x4* const at = reinterpret_cast<f32x4*>(sO + n32 * (DP + 4) + 32 * d + 8 * g + 4 * hi);
-          f32x4 x = {o[d][4 * g] * mine, o[d][4 * g + 1] * mine, o[d][4 * g + 2] * mine, o[d][4 * g + 3] * mine};
-          if (m == -RB_INF) x = f32x4{0.f, 0.f, 0.f, 0.f};
-          *at = w == 0 ? x : *at + x;
-        }
-    }
-    __syncthreads();
-  }
-  if (wave == 0 && hi == 0) sM[n32] = mall, sM[32 + n32] = valid ? lall : 0.f;
+    for (int e = 0; e < 4; ++e)
+      *reinterpret_cast<f32x4*>(sO + (wave * 32 + n32) * (DP + 4) + 32 * d + 8 * e + 4 * hi) =
+          f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
   __syncthreads();
   const int rows = min(32, R - rb * 32);
-  if (a.nsplit == 1) {
-    for (int x = tid; x < rows * (DP / 4); x += 256) {
-      const int r = x / (DP / 4), c = x % (DP / 4) * 4, rr = rb * 32 + r;
-      if (c >= a.D) continue;
-      const float sum = sM[32 + r], inv = 1.f / sum;
-      const f32x4 y = *reinterpret_cast<const f32x4*>(sO + r * (DP + 4) + c);
-      uint16_t* const op = a.out + b * a.so.b + (int64_t)(rr / G) * a.so.t + (hk * G + rr % G) * a.so.h + c;
+  const int64_t first = (int64_t)bk * R + rb * 32;
+  float2* const ml = reinterpret_cast<float2*>(a.part + (int64_t)a.B * a.Hk * R * a.nsplit * DP);
+  for (int x = tid; x < rows * (DP / 4); x += NT) {
+    const int r = x / (DP / 4), c = x % (DP / 4) * 4, rr = rb * 32 + r;
+    float top = -RB_INF, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) top = fmaxf(top, sM[w * 64 + r]);
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {  // in order
+      const float lw = sM[w * 64 + 32 + r];
+      if (lw == 0.f) continue;
+      const float f = __builtin_amdgcn_exp2f((sM[w * 64 + r] - top) * a.c2);
+      sum += lw * f;
+      y += *reinterpret_cast<const f32x4*>(sO + (w * 32 + r) * (DP + 4) + c) * f;
+    }
+    if (a.nsplit > 1) {  // O rows [row][split][DP], then (reference, sum) [row][split]
+      *reinterpret_cast<f32x4*>(a.part + ((first + r) * a.nsplit + split) * DP + c) = y;
+      if (c == 0) ml[(first + r) * a.nsplit + split] = make_float2(top * a.c2, sum);
+      continue;
+    }
+    const int64_t hq = hk * G + rr % G, iq = rr / G;
+    if (c < a.D) {
+      uint16_t* const op = a.out + b * a.so.b + iq * a.so.t + hq * a.so.h + c;
+      const float inv = 1.f / sum;
       if (sum == 0.f) store4<E>(op, 0.f, 0.f, 0.f, 0.f);
       else store4<E>(op, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
     }
-    if (a.lse != nullptr && tid < rows) {
-      const int rr = rb * 32 + tid;
-      const float sum = sM[32 + tid];
-      a.lse[((int64_t)b * a.H + hk * G + rr % G) * a.Tq + rr / G] =
-          sum == 0.f ? -RB_INF : (sM[tid] * a.c2 + __builtin_amdgcn_logf(sum)) * RB_LN2;
-    }
-    return;
+    if (c == 0 && a.lse != nullptr)
+      a.lse[((int64_t)b * a.H + hq) * a.Tq + iq] = sum == 0.f ? -RB_INF : (top * a.c2 + __builtin_amdgcn_logf(sum)) * RB_LN2;
   }
-  // workspace: O rows [row][split][DP], then (reference, sum) [row][split]
-  const int64_t first = (int64_t)bk * R + rb * 32;
-  for (int x = tid; x < rows * (DP / 4); x += 256) {
-    const int r = x / (DP / 4), c = x % (DP / 4) * 4;
-    *reinterpret_cast<f32x4*>(a.part + ((first + r) * a.nsplit + split) * DP + c) = *reinterpret_cast<const f32x4*>(sO + r * (DP + 4) + c);
-  }
-  float2* const ml = reinterpret_cast<float2*>(a.part + (int64_t)a.B * a.Hk * R * a.nsplit * DP);
-  if (tid < rows) ml[(first + tid) * a.nsplit + split] = make_float2(sM[tid] * a.c2, sM[32 + tid]);
 }
 
 // one wave per row: the splits' states in order, 64 at a time (their weights in the lanes, so that the loads of O do not wait)
@@ -1139,11 +1143,11 @@ size_t dkv_lds(int DP, int md) { return fwd_lds(DP, md) + 1024; }
 
 // launches with more than 64 KB of LDS have to be allowed, per device: asked for at each such launch
 template <class K>
-int launch(K kernel, int64_t blocks, size_t lds, const RbArgs& a, hipStream_t s) {
+int launch(K kernel, int64_t blocks, size_t lds, const RbArgs& a, hipStream_t s, int threads = 256) {
   if (lds > 64 * 1024 &&
       hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
     return CSSHIP_ELAUNCH;
-  kernel<<<(unsigned)blocks, 256, lds, s>>>(a);
+  kernel<<<(unsigned)blocks, threads, lds, s>>>(a);
   CSSHIP_CHECK_LAUNCH();
   return CSSHIP_OK;
 }
@@ -1169,8 +1173,11 @@ int launch_fwd(RbArgs a, const csship_relbias* p, hipStream_t s) {
     a.ntile = f.ntile;
     a.nsplit = f.nsplit;
     a.nblk = a.B * a.Hk * a.ntile * a.nsplit;
-    const size_t tiles = 4 * 32 * 2 * DP, join = (32 * (DP + 4) + 256) * 4;
-    if (const int rc = launch(rb_few_kernel<E, DP>, a.nblk, tiles > join ? tiles : join, a, s)) return rc;
+    const int table = (a.H / a.Hk) * (2 * a.mde + 1), staged = table <= RB_FEW_TABLE ? table * 4 : 0;
+    // few workgroups: twice the waves, half the tiles for each (1 x 500 keys, 4 heads: FEWUS)
+    const int rc = a.nblk < 256 ? launch(rb_few_kernel<E, DP, 8>, a.nblk, few_area<DP, 8>() + staged, a, s, 512)
+                                : launch(rb_few_kernel<E, DP, 4>, a.nblk, few_area<DP, 4>() + staged, a, s);
+    if (rc) return rc;
     if (a.nsplit == 1) return CSSHIP_OK;
     return launch(rb_join_kernel<E, DP>, ((int64_t)a.B * a.H * a.Tq + 3) / 4, 0, a, s);
   }

@@ -404,13 +404,13 @@ def mha_relbias(q, k, v, table, buckets, *, scale=None, causal=False, offset=0, 
             return mha_relbias(q, k, v, table, buckets, scale=scale, causal=causal, offset=offset, k_lens=k_lens, q_lens=q_lens,
                                want_lse=want_lse)
     B, Tq, H, _ = q.shape
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((B, H, Tq), dtype=torch.float32, device=q.device) if want_lse else None
     h = lib()
     n = h.csship_relbias_fwd_workspace(p)
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     check(h.csship_relbias_fwd(p, out.data_ptr(), _strides3(out), lse.data_ptr() if want_lse else None,
-                               ws.data_ptr() if n else None, n, torch.cuda.current_stream(at).cuda_stream))
+                               ws.data_ptr() if n else None, n, torch._C._cuda_getCurrentRawStream(at)))
     return (out, lse) if want_lse else out
 
 

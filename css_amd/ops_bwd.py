@@ -819,15 +819,13 @@ def mha_relbias_bwd(q, k, v, table, out, lse, dout, buckets, *, scale=None, caus
             return mha_relbias_bwd(q, k, v, table, out, lse, dout, buckets, scale=scale, causal=causal, offset=offset,
                                    k_lens=k_lens, q_lens=q_lens)
     lse = lse.contiguous()
-    dq = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device)
-    dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
-    dtable = torch.empty(table.shape, dtype=torch.float32, device=q.device)
+    dq, dk, dv, dtable = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v, table))
     h = lib()
     ws = torch.empty(h.csship_relbias_bwd_workspace(p), dtype=torch.uint8, device=q.device)
     s3 = ops._strides3
     check(h.csship_relbias_bwd(p, out.data_ptr(), s3(out), lse.data_ptr(), dout.data_ptr(), s3(dout), dq.data_ptr(), s3(dq),
                                dk.data_ptr(), s3(dk), dv.data_ptr(), s3(dv), dtable.data_ptr(), ws.data_ptr(), ws.numel(),
-                               torch.cuda.current_stream(at).cuda_stream))
+                               torch._C._cuda_getCurrentRawStream(at)))
     return dq, dk, dv, dtable
 
 
