@@ -99,6 +99,10 @@ DEV int xcd_order(int id, int n) {
   return x * full + min(x, rest) + i;
 }
 
+// Causal rows: the last tiles are the longest, and start first.  Every second 256 workgroups the order turns round: a CU that took a
+// long one of the first 256 gets a short one of the next (both sit on it at once).
+DEV int row_tile(const RbArgs& a, int rank) { return a.causal && ((blockIdx.x >> 8) & 1) ? rank : a.ntile - 1 - rank; }
+
 // table entry -> score units (the products' accumulators hold q . k, scaled later by c2)
 DEV float bias_units(const RbArgs& a, float w) { return w <= -RB_BIG ? -RB_INF : (w > RB_BIG ? RB_BIG : w) * a.inv_scale; }
 DEV float bias_entry(const RbArgs& a, int r, int h) { return bias_units(a, a.table[a.bucket_of[r + a.md] * a.H + h]); }
@@ -258,7 +262,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
   float* const sB = reinterpret_cast<float*>(smem + 4 * TILE);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const int id = xcd_order(blockIdx.x, a.nblk);
-  const int bh = id / a.ntile, tile = a.ntile - 1 - id % a.ntile;  // a causal row's last tiles are the longest: first
+  const int bh = id / a.ntile, tile = row_tile(a, id % a.ntile);
   const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
   const Seq sq = seq_of(a, b);
   const int q0 = tile * 128, i = q0 + wave * 32 + n32, p0 = sq.off + q0 + wave * 32;
@@ -668,7 +672,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   double* const sFar = reinterpret_cast<double*>(smem + 4 * TILE + ((9 * span + 1) / 2 * 2) * 4);  // [4][2], [4]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const int id = xcd_order(blockIdx.x, a.nblk);
-  const int bh = id / a.ntile, tile = a.ntile - 1 - id % a.ntile;
+  const int bh = id / a.ntile, tile = row_tile(a, id % a.ntile);
   const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
   const Seq sq = seq_of(a, b);
   const int q0 = tile * 128, i = q0 + wave * 32 + n32, p0 = sq.off + q0 + wave * 32;

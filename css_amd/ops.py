@@ -405,7 +405,7 @@ def mha_relbias(q, k, v, table, buckets, *, scale=None, causal=False, offset=0, 
                                want_lse=want_lse)
     B, Tq, H, _ = q.shape
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty((B, H, Tq), dtype=torch.float32, device=q.device) if want_lse else None
+    lse = table.new_empty((B, H, Tq)) if want_lse else None
     h = lib()
     n = h.csship_relbias_fwd_workspace(p)
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
