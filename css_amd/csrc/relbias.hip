@@ -55,7 +55,26 @@ struct ElemHf {
 
 struct Strides { int64_t b, t, h; };  // elements
 
+// division of 0 <= n < 2^31 by a number known on the host: n mul >> shift, exact (mul = ceil(2^shift / d), shift = 31 + ceil(log2 d))
+struct Divisor {
+  unsigned mul, shift;
+  int d;
+  void set(int by) {
+    d = by;
+    shift = 31;
+    while ((1ll << (shift - 31)) < by) ++shift;
+    mul = (unsigned)(((1ull << shift) + (unsigned)by - 1) / (unsigned)by);
+  }
+  __device__ __forceinline__ int over(int n) const { return (int)(((uint64_t)(unsigned)n * mul) >> shift); }
+};
+struct Quot { int q, r; };
+DEV Quot split(int n, const Divisor& d) {
+  const int q = d.over(n);
+  return Quot{q, n - q * d.d};
+}
+
 struct RbArgs {
+  Divisor per_tile, per_head, per_group, per_split;  // ntile; H or Hk, as the kernel counts; H / Hk; nsplit
   const uint16_t *q, *k, *v, *o, *dout;
   Strides sq, sk, sv, so, sdo, sdq, sdk, sdv;
   const float* table;
@@ -262,8 +281,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
   float* const sB = reinterpret_cast<float*>(smem + 4 * TILE);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const int id = xcd_order(blockIdx.x, a.nblk);
-  const int bh = id / a.ntile, tile = row_tile(a, id % a.ntile);
-  const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
+  const Quot it = split(id, a.per_tile), bh = split(it.q, a.per_head);
+  const int b = bh.q, h = bh.r, hk = a.per_group.over(h), tile = row_tile(a, it.r);
   const Seq sq = seq_of(a, b);
   const int q0 = tile * 128, i = q0 + wave * 32 + n32, p0 = sq.off + q0 + wave * 32;
   int kend = q0 < sq.qlen ? sq.klen : 0, wend = q0 + wave * 32 < sq.qlen ? sq.klen : 0;
@@ -428,18 +447,19 @@ __global__ __launch_bounds__(64 * NW, 2) void rb_few_kernel(RbArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   unsigned char* const sV = smem + wave * 32 * P;
   float* const sT = reinterpret_cast<float*>(smem + few_area<DP, NW>());
-  const int G = a.H / a.Hk, R = a.Tq * G;
+  const int G = a.per_group.d, R = a.Tq * G;
   const int id = xcd_order(blockIdx.x, a.nblk);
-  const int split = id % a.nsplit, rb = id / a.nsplit % a.ntile, bk = id / a.nsplit / a.ntile;
-  const int b = bk / a.Hk, hk = bk % a.Hk;
+  const Quot is = split(id, a.per_split), it = split(is.q, a.per_tile), bh = split(it.q, a.per_head);
+  const int part = is.r, rb = it.r, bk = it.q, b = bh.q, hk = bh.r;
   const Seq sq = seq_of(a, b);
-  const int row = rb * 32 + n32, i = row / G, g = row - i * G, h = hk * G + g;
+  const Quot ig = split(rb * 32 + n32, a.per_group);
+  const int row = rb * 32 + n32, i = ig.q, g = ig.r, h = hk * G + g;
   const bool valid = row < R && i < sq.qlen;
-  const int p = sq.off + i, i_last = min((rb * 32 + 31) / G, sq.qlen - 1);
-  int kend = rb * 32 / G < sq.qlen ? sq.klen : 0;
+  const int p = sq.off + i, i_first = a.per_group.over(rb * 32), i_end = a.per_group.over(rb * 32 + 31), i_last = min(i_end, sq.qlen - 1);
+  int kend = i_first < sq.qlen ? sq.klen : 0;
   if (a.causal) kend = min(kend, sq.off + i_last + 1);
-  const int ntile = kend > 0 ? (kend + 31) >> 5 : 0, per = (ntile + a.nsplit - 1) / a.nsplit;
-  const int t0 = split * per, t1 = min(ntile, t0 + per);
+  const int ntile = kend > 0 ? (kend + 31) >> 5 : 0, per = a.per_split.over(ntile + a.nsplit - 1);
+  const int t0 = part * per, t1 = min(ntile, t0 + per);
   const uint16_t* const kp = a.k + b * a.sk.b + hk * a.sk.h;
   const uint16_t* const vp = a.v + b * a.sv.b + hk * a.sv.h;
 
@@ -475,7 +495,7 @@ __global__ __launch_bounds__(64 * NW, 2) void rb_few_kernel(RbArgs a) {
   }
   const int hc = hk * G + min(g, G - 1);
   const float left = bias_entry(a, -a.mde, hc), right = bias_entry(a, a.mde, hc);
-  const int p_lo = sq.off + rb * 32 / G, p_hi = sq.off + (rb * 32 + 31) / G;  // positions of the workgroup's rows
+  const int p_lo = sq.off + i_first, p_hi = sq.off + i_end;  // positions of the workgroup's rows
   // the group's tables by distance, if any tile of the workgroup's needs them
   const int wide = 2 * a.mde + 1;
   const bool staged = G * wide <= RB_FEW_TABLE;
@@ -573,8 +593,8 @@ __global__ __launch_bounds__(64 * NW, 2) void rb_few_kernel(RbArgs a) {
       y += *reinterpret_cast<const f32x4*>(sO + (w * 32 + r) * (DP + 4) + c) * f;
     }
     if (a.nsplit > 1) {  // O rows [row][split][DP], then (reference, sum) [row][split]
-      *reinterpret_cast<f32x4*>(a.part + ((first + r) * a.nsplit + split) * DP + c) = y;
-      if (c == 0) ml[(first + r) * a.nsplit + split] = make_float2(top * a.c2, sum);
+      *reinterpret_cast<f32x4*>(a.part + ((first + r) * a.nsplit + part) * DP + c) = y;
+      if (c == 0) ml[(first + r) * a.nsplit + part] = make_float2(top * a.c2, sum);
       continue;
     }
     const int64_t hq = hk * G + rr % G, iq = rr / G;
@@ -672,8 +692,8 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   double* const sFar = reinterpret_cast<double*>(smem + 4 * TILE + ((9 * span + 1) / 2 * 2) * 4);  // [4][2], [4]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const int id = xcd_order(blockIdx.x, a.nblk);
-  const int bh = id / a.ntile, tile = row_tile(a, id % a.ntile);
-  const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
+  const Quot it = split(id, a.per_tile), bh = split(it.q, a.per_head);
+  const int b = bh.q, h = bh.r, hk = a.per_group.over(h), tile = row_tile(a, it.r);
   const Seq sq = seq_of(a, b);
   const int q0 = tile * 128, i = q0 + wave * 32 + n32, p0 = sq.off + q0 + wave * 32;
   int kend = q0 < sq.qlen ? sq.klen : 0, wend = q0 + wave * 32 < sq.qlen ? sq.klen : 0;
@@ -928,8 +948,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
   float* const sB = sL + 256;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const int id = xcd_order(blockIdx.x, a.nblk);
-  const int split = id % a.nsplit, bh = id / a.nsplit / a.ntile, tile = id / a.nsplit % a.ntile;
-  const int b = bh / a.Hk, hk = bh % a.Hk, G = a.H / a.Hk;
+  const Quot is = split(id, a.per_split), it_ = split(is.q, a.per_tile), bh = split(it_.q, a.per_head);
+  const int part = is.r, tile = it_.r, b = bh.q, hk = bh.r, G = a.per_group.d;
   const Seq sq = seq_of(a, b);
   const int k0 = tile * 128, j0 = k0 + wave * 32, j = j0 + n32;
   u32x4 kf[NK], vf[NK];
@@ -941,7 +961,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
   // causal: the first query that sees key k0 sits at position k0.  Steps are numbered head by head.
   const int t0 = a.causal ? max(k0 - sq.off, 0) >> 6 : 0;
   const int per = k0 < sq.klen ? max(((sq.qlen + 63) >> 6) - t0, 0) : 0, steps = per * G;
-  const int it0 = (int)((int64_t)steps * split / a.nsplit), it1 = (int)((int64_t)steps * (split + 1) / a.nsplit);
+  const int it0 = (int)((int64_t)steps * part / a.nsplit), it1 = (int)((int64_t)steps * (part + 1) / a.nsplit);
   const unsigned lQ = lds_addr(sQ), lO = lds_addr(sO);
   float lrow = 0.f;
 
@@ -1049,7 +1069,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
   if (j >= a.Tk) return;
   if (a.nsplit > 1) {  // sums in f32: [split][dk | dv][sequence, key head, key][DP]
     const int64_t rows = (int64_t)a.B * a.Hk * a.Tk, row = ((int64_t)b * a.Hk + hk) * a.Tk + j;
-    float* const pk = a.part2 + ((int64_t)split * 2 * rows + row) * DP;
+    float* const pk = a.part2 + ((int64_t)part * 2 * rows + row) * DP;
     float* const pv = pk + rows * DP;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -1147,7 +1167,11 @@ size_t dkv_lds(int DP, int md) { return fwd_lds(DP, md) + 1024; }
 
 // launches with more than 64 KB of LDS have to be allowed, per device: asked for at each such launch
 template <class K>
-int launch(K kernel, int64_t blocks, size_t lds, const RbArgs& a, hipStream_t s, int threads = 256) {
+int launch(K kernel, int64_t blocks, size_t lds, RbArgs a, int heads, hipStream_t s, int threads = 256) {
+  a.per_tile.set(a.ntile < 1 ? 1 : a.ntile);
+  a.per_head.set(heads);
+  a.per_group.set(a.H / a.Hk);
+  a.per_split.set(a.nsplit < 1 ? 1 : a.nsplit);
   if (lds > 64 * 1024 &&
       hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
     return CSSHIP_ELAUNCH;
@@ -1179,16 +1203,16 @@ int launch_fwd(RbArgs a, const csship_relbias* p, hipStream_t s) {
     a.nblk = a.B * a.Hk * a.ntile * a.nsplit;
     const int table = (a.H / a.Hk) * (2 * a.mde + 1), staged = table <= RB_FEW_TABLE ? table * 4 : 0;
     // few workgroups: twice the waves, half the tiles for each (1 x 500 keys, 4 heads: FEWUS)
-    const int rc = a.nblk < 256 ? launch(rb_few_kernel<E, DP, 8>, a.nblk, few_area<DP, 8>() + staged, a, s, 512)
-                                : launch(rb_few_kernel<E, DP, 4>, a.nblk, few_area<DP, 4>() + staged, a, s);
+    const int rc = a.nblk < 256 ? launch(rb_few_kernel<E, DP, 8>, a.nblk, few_area<DP, 8>() + staged, a, a.Hk, s, 512)
+                                : launch(rb_few_kernel<E, DP, 4>, a.nblk, few_area<DP, 4>() + staged, a, a.Hk, s);
     if (rc) return rc;
     if (a.nsplit == 1) return CSSHIP_OK;
-    return launch(rb_join_kernel<E, DP>, ((int64_t)a.B * a.H * a.Tq + 3) / 4, 0, a, s);
+    return launch(rb_join_kernel<E, DP>, ((int64_t)a.B * a.H * a.Tq + 3) / 4, 0, a, a.H, s);
   }
   a.ntile = (a.Tq + 127) / 128;
   a.nblk = a.B * a.H * a.ntile;
   if (a.nblk == 0) return CSSHIP_OK;
-  return launch(rb_fwd_kernel<E, DP>, a.nblk, fwd_lds(DP, a.mde), a, s);
+  return launch(rb_fwd_kernel<E, DP>, a.nblk, fwd_lds(DP, a.mde), a, a.H, s);
 }
 
 // Workgroups of the dk / dv kernel take 128 keys of a sequence and key head; where those leave most of the chip idle, each one's
@@ -1206,14 +1230,14 @@ int launch_bwd(RbArgs a, const csship_relbias* p, hipStream_t s) {
   a.tq128 = a.ntile * 128;
   a.nblk = a.B * a.H * a.ntile;
   if (a.nblk > 0)
-    if (const int rc = launch(rb_dq_kernel<E, DP>, a.nblk, dq_lds(DP, a.mde), a, s)) return rc;
+    if (const int rc = launch(rb_dq_kernel<E, DP>, a.nblk, dq_lds(DP, a.mde), a, a.H, s)) return rc;
   a.ntile = (a.Tk + 127) / 128;
   a.nsplit = dkv_splits(p);
   a.nblk = a.B * a.Hk * a.ntile * a.nsplit;
   const int64_t entries = ((int64_t)a.nb * a.H + 3) / 4;
-  if (const int rc = launch(rb_dkv_kernel<E, DP>, a.nblk > entries ? a.nblk : entries, dkv_lds(DP, a.mde), a, s)) return rc;
+  if (const int rc = launch(rb_dkv_kernel<E, DP>, a.nblk > entries ? a.nblk : entries, dkv_lds(DP, a.mde), a, a.Hk, s)) return rc;
   if (a.nsplit == 1) return CSSHIP_OK;
-  return launch(rb_dkv_join_kernel<E, DP>, ((int64_t)2 * a.B * a.Hk * a.Tk * (DP / 4) + 255) / 256, 0, a, s);
+  return launch(rb_dkv_join_kernel<E, DP>, ((int64_t)2 * a.B * a.Hk * a.Tk * (DP / 4) + 255) / 256, 0, a, a.Hk, s);
 }
 
 template <class E>
