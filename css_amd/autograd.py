@@ -178,6 +178,34 @@ class PitMse(torch.autograd.Function):
         return (g,) + (None,) * (2 + len(targets))
 
 
+class MhaRelBias(torch.autograd.Function):
+    """ops.mha_relbias with ops_bwd.mha_relbias_bwd behind it; keeps q, k, v, the table, out and the rows' log-sum-exp."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, table, buckets, scale, causal, offset, k_lens, q_lens):
+        out, lse = ops.mha_relbias(q, k, v, table, buckets, scale=scale, causal=causal, offset=offset, k_lens=k_lens,
+                                   q_lens=q_lens, want_lse=True)
+        each = isinstance(offset, torch.Tensor)
+        ctx.save_for_backward(q, k, v, table, out, lse, offset if each else None, k_lens, q_lens)
+        ctx.how = (buckets, scale, causal, None if each else offset)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, table, out, lse, offsets, k_lens, q_lens = ctx.saved_tensors
+        buckets, scale, causal, offset = ctx.how
+        grads = ob.mha_relbias_bwd(q, k, v, table, out, lse, dout, buckets, scale=scale, causal=causal,
+                                        offset=offset if offsets is None else offsets, k_lens=k_lens, q_lens=q_lens)
+        return (*grads, None, None, None, None, None, None)
+
+
+def mha_relbias(q, k, v, table, buckets, *, scale=None, causal=False, offset=0, k_lens=None, q_lens=None):
+    """ops.mha_relbias under autograd: out, differentiable in q, k, v and the bias table (arguments as there).  Rows behind a
+    sequence's end get zero gradients, whatever arrives from above for them."""
+    return MhaRelBias.apply(q, k, v, table, buckets, scale, causal, offset, k_lens, q_lens)
+
+
 def _conformer_pack_plan(model, wide, device):
     """bf16 shadows (row-major / MFMA fragment order / fragment-packed transposes) of every Linear weight of the model,
     produced by ONE launch per step.  Built once per (model, kernel family, device); the destinations are rewritten in

@@ -34,6 +34,7 @@ using True = Const<1>;
 using False = Const<0>;
 
 struct ElemBf {
+  static constexpr bool narrow = false;  // exponents as wide as f32's
   DEV f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -41,7 +42,11 @@ struct ElemBf {
   DEV float lo(unsigned u) { return __uint_as_float(u << 16); }
   DEV float hi(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
 };
+// fp16 reaches down to 2^-24 only.  P is at most 1 and what rounds to zero there is below 2^-25 of its row; dS has the size of
+// the incoming gradient, which may be far smaller than 1: it is multiplied by a power of two before it is rounded, and the
+// sums are divided by it (row_factor).
 struct ElemHf {
+  static constexpr bool narrow = true;
   DEV f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -84,7 +89,7 @@ struct RbArgs {
   uint16_t *out, *dq, *dk, *dv;
   float *lse, *dtable;
   const float* lse_in;
-  float *delta, *lse2, *part, *part2;  // workspace; delta (negated) and lse2 [B, H, tq128]
+  float *delta, *lse2, *size, *part, *part2;  // workspace; delta (negated), lse2, size (sum of squares of dout's row) [B, H, tq128]
   int B, Tq, Tk, H, Hk, D, nb, md, mde, causal, offset;  // mde: md, or the furthest distance that occurs
   float scale, inv_scale, c2;  // c2 = scale * log2(e)
   int ntile, nblk, nsplit, nqtile, tq128;     // row tiles per (sequence, head); workgroups; key ranges (rb_few_kernel)
@@ -163,6 +168,11 @@ DEV float half_sum(float x) {
   return __uint_as_float(a0) + __uint_as_float(a1);
 }
 
+// the power of two that brings a row of dout with this sum of squares to a norm of 1 .. 2 (1 for zeros and for what is not finite)
+DEV float row_factor(float squares) {
+  const int e = (int)((__float_as_uint(squares) >> 23) & 0xff) - 127;  // floor(log2)
+  return squares > 0.f && e < 128 ? __uint_as_float((unsigned)(127 - (max(min(e, 120), -120) >> 1)) << 23) : 1.f;
+}
 DEV double wave_total(double x) {
 #pragma unroll
   for (int w = 1; w < 64; w <<= 1) x += __shfl_xor(x, w);
@@ -714,7 +724,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   u32x4 qf[NK], df[NK];
   row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, q0 + wave * 32, sq.qlen, a.D, lane, qf);
   row_frags<DP>(a.dout + b * a.sdo.b + h * a.sdo.h, a.sdo.t, q0 + wave * 32, sq.qlen, a.D, lane, df);
-  float delta = 0.f, lse2 = RB_INF;
+  float delta = 0.f, lse2 = RB_INF, fac = 1.f;  // fac: of the rounded dS (fp16)
   {
     u32x4 of[NK];
     row_frags<DP>(a.o + b * a.so.b + h * a.so.h, a.so.t, q0 + wave * 32, sq.qlen, a.D, lane, of);
@@ -726,6 +736,16 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) delta += E::lo(df[ks][e]) * E::lo(of[ks][e]) + E::hi(df[ks][e]) * E::hi(of[ks][e]);
     delta = half_sum(delta);
+    if constexpr (E::narrow) {
+      float squares = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < NK; ++ks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) squares += E::lo(df[ks][e]) * E::lo(df[ks][e]) + E::hi(df[ks][e]) * E::hi(df[ks][e]);
+      squares = half_sum(squares);
+      fac = row_factor(squares);
+      if (hi == 0) a.size[((int64_t)b * a.H + h) * a.tq128 + i] = squares;
+    }
     if (x != -RB_INF) lse2 = x * RB_LOG2E;
     const int64_t to = ((int64_t)b * a.H + h) * a.tq128 + i;  // rows up to the tile's end: the next kernel reads whole tiles
     if (hi == 0) a.delta[to] = -delta, a.lse2[to] = lse2;
@@ -836,6 +856,10 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
         if (j0 > p0) farr += y;
         else farl += y;
       }
+      if constexpr (E::narrow) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= fac;
+      }
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         const u32x4 ds = pack8<E>(s, 8 * kk);
@@ -862,13 +886,13 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
 
   if (i < a.Tq) {
     uint16_t* const op = a.dq + b * a.sdq.b + (int64_t)i * a.sdq.t + h * a.sdq.h;
+    const float f = E::narrow ? a.scale / fac : a.scale;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int c = 32 * d + 8 * g + 4 * hi;
-        if (c < a.D)
-          store4<E>(op + c, dq[d][4 * g] * a.scale, dq[d][4 * g + 1] * a.scale, dq[d][4 * g + 2] * a.scale, dq[d][4 * g + 3] * a.scale);
+        if (c < a.D) store4<E>(op + c, dq[d][4 * g] * f, dq[d][4 * g + 1] * f, dq[d][4 * g + 2] * f, dq[d][4 * g + 3] * f);
       }
   }
   // The workgroup's share of the table's gradient.  A bucket's distances are contiguous: running sums over the distances in 64
@@ -945,7 +969,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
   unsigned char* const sQ = smem;
   unsigned char* const sO = smem + 2 * TILE;
   float* const sL = reinterpret_cast<float*>(smem + 4 * TILE);  // [2][2][64] lse2 | -delta of a tile's rows
-  float* const sB = sL + 256;
+  float* const sF = sL + 256;                                   // [2] largest sum of squares of a tile's rows of dout (fp16)
+  float* const sB = sF + 4;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const int id = xcd_order(blockIdx.x, a.nblk);
   const Quot is = split(id, a.per_split), it_ = split(is.q, a.per_tile), bh = split(it_.q, a.per_head);
@@ -963,7 +988,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
   const int per = k0 < sq.klen ? max(((sq.qlen + 63) >> 6) - t0, 0) : 0, steps = per * G;
   const int it0 = (int)((int64_t)steps * part / a.nsplit), it1 = (int)((int64_t)steps * (part + 1) / a.nsplit);
   const unsigned lQ = lds_addr(sQ), lO = lds_addr(sO);
-  float lrow = 0.f;
+  float lrow = 0.f, fac = 2e37f;  // fac (fp16): above every factor until a gradient has been seen
 
   for (int it = it0; it < it1;) {
     const int g = it / per, ta = t0 + it % per, tb = min(t0 + per, ta + it1 - it);  // one head's run of tiles
@@ -972,14 +997,19 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
     TileDma<DP> dQ, dO;
     dQ.init(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, ta, sq.qlen, a.D, wave, lane);
     dO.init(a.dout + b * a.sdo.b + h * a.sdo.h, a.sdo.t, ta, sq.qlen, a.D, wave, lane);
-    const float* const rl = (wave == 0 ? a.lse2 : a.delta) + ((int64_t)b * a.H + h) * a.tq128;
+    constexpr int ROWS = E::narrow ? 3 : 2;  // waves that bring a tile's row statistics
+    const float* const rl = (wave == 0 ? a.lse2 : wave == 1 ? a.delta : a.size) + ((int64_t)b * a.H + h) * a.tq128;
     auto load = [&](int t, int buf) {
       dQ.next(lQ + buf * TILE, wave);
       dO.next(lO + buf * TILE, wave);
-      if (wave < 2) lrow = rl[t * 64 + lane];
+      if (wave < ROWS) lrow = rl[t * 64 + lane];
     };
     auto store = [&](int buf) {
       if (wave < 2) sL[buf * 128 + wave * 64 + lane] = lrow;
+      if (E::narrow && wave == 2) {
+        const float top = wave_max(lrow);
+        if (lane == 0) sF[buf] = top;
+      }
     };
     __syncthreads();  // the head before has been read
     load(ta, 0);
@@ -995,6 +1025,17 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
       const unsigned char* const qt = sQ + buf * TILE;
       const unsigned char* const ot = sO + buf * TILE;
       const float* const lt = sL + buf * 128;
+      if constexpr (E::narrow) {  // one factor for all of dK's sum so far: a tile of larger gradients takes it down
+        const float top = sF[buf], f = row_factor(top);
+        if (top > 0.f && f < fac) {
+          const float down = fac > 1e37f ? 0.f : f / fac;
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dk[d][r] *= down;
+          fac = f;
+        }
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int p0 = sq.off + t * 64 + 32 * u;  // position of the sub-tile's first query
@@ -1051,7 +1092,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, -ls[r >> 2][r & 3]));
-          dp[r] *= s[r];
+          dp[r] *= E::narrow ? s[r] * fac : s[r];
         }
         outer(ot, s, dv);
         outer(qt, dp, dk);
@@ -1064,6 +1105,13 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
       step(t, Const<0>{});
       if (t + 1 < tb) step(t + 1, Const<1>{});
     }
+  }
+  if constexpr (E::narrow) {
+    const float f = 1.f / fac;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dk[d][r] *= f;
   }
   table_sum(a, blockIdx.x * 4 + wave, a.B * a.nqtile);  // each wave one entry of the table's gradient, from the dq kernel's shares
   if (j >= a.Tk) return;
@@ -1163,7 +1211,7 @@ RbArgs to_args(const csship_relbias* p) {
 
 size_t fwd_lds(int DP, int md) { return (size_t)4 * 64 * 2 * DP + (2 * (md + RB_PAD) + 1) * 4; }
 size_t dq_lds(int DP, int md) { return (size_t)4 * 64 * 2 * DP + (size_t)(9 * (2 * (md + RB_PAD) + 1) + 1) / 2 * 2 * 4 + 96; }
-size_t dkv_lds(int DP, int md) { return fwd_lds(DP, md) + 1024; }
+size_t dkv_lds(int DP, int md) { return fwd_lds(DP, md) + 1024 + 16; }
 
 // launches with more than 64 KB of LDS have to be allowed, per device: asked for at each such launch
 template <class K>
@@ -1286,7 +1334,7 @@ size_t csship_relbias_bwd_workspace(const csship_relbias* p) {
   if (check_args(p) != CSSHIP_OK) return 0;
   const int splits = dkv_splits(p);
   const int64_t sums = splits == 1 ? 0 : (int64_t)splits * 2 * p->B * p->Hk * p->Tk * width_of(p->D);
-  return (size_t)(2 * row_words(p) + part_words(p) + sums) * 4 + 16;
+  return (size_t)(3 * row_words(p) + part_words(p) + sums) * 4 + 16;
 }
 
 int csship_relbias_bwd(const csship_relbias* p, const uint16_t* out, const int64_t* out_stride, const float* lse, const uint16_t* dout,
@@ -1314,7 +1362,8 @@ int csship_relbias_bwd(const csship_relbias* p, const uint16_t* out, const int64
   a.dtable = dtable;
   a.delta = static_cast<float*>(workspace);
   a.lse2 = a.delta + row_words(p);
-  a.part = a.lse2 + row_words(p);
+  a.size = a.lse2 + row_words(p);
+  a.part = a.size + row_words(p);
   a.part2 = a.part + part_words(p);
   return p->dtype == CSSHIP_RELBIAS_BF16 ? bwd_by_width<ElemBf>(a, p, as_stream(stream)) : bwd_by_width<ElemHf>(a, p, as_stream(stream));
 }

@@ -257,6 +257,161 @@ def test_same_bits_every_time(lib):
         assert all(torch.equal(a, b) for a, b in zip(first, got))
 
 
+def test_small_gradients_in_fp16(lib):
+    """dS has the size of the incoming gradient: 2^-14 here, and a thousandth of that per key.  Rounded as it is, dS would lie among
+    fp16's subnormals (relative error 10^-2 and more); roundings to full precision are independent, u / sqrt(3) each at most
+    on average, and dq and dk are rounded twice: below 2 u = 2^-10 in the 2-norm.  One head's gradient comes 2^12 larger from query
+    150 on: the running factor of dk goes down in the middle of the sum."""
+    ops, ob = lib
+    q, k, v, table, do = make(9, torch.float16, 1, 300, 200, 2, 1, 64, 32)
+    k = (k * 8).half()
+    q = (q / 8).half()
+    for late in (1.0, 4096.0):
+        d = do.float() * 2.0 ** -14
+        d[:, 150:, 1] *= late
+        d = d.half()
+        out, lse = ops.mha_relbias(q, k, v, table, (32, 128), want_lse=True)
+        got = dict(zip(("dq", "dk", "dv", "dtable"), ob.mha_relbias_bwd(q, k, v, table, out, lse, d, (32, 128))))
+        ref, _ = reference(q, k, v, table, (32, 128), dout=d, out=out)
+        # dq, in multiples of what fp16 can hold at this size: its own subnormals are the caller's choice of scale
+        for name in ("dq", "dk"):
+            want = ref[name]
+            floor = want.numel() ** 0.5 * 2.0 ** -25
+            assert float((got[name].cpu().double() - want).norm()) < 2.0 ** -10 * float(want.norm()) + floor, (name, late)
+        off = (got["dtable"].cpu().double() - ref["dtable"]).norm() / ref["dtable"].norm()
+        assert float(off) < 2e-5
+
+
+def test_cache_beyond_32_bit_offsets(lib):
+    """keys and values as the last heads of a cache of 5.2 GB: element offsets above 2^31, in both forward forms and the backward"""
+    B, T, D = 1, 5200, 128
+    cache = torch.empty(B, T, 3904, D, dtype=torch.bfloat16, device=DEV)
+    cache[:, :, 3902:] = torch.randn(B, T, 2, D, device=DEV).bfloat16()
+    k, v = cache[:, :, 3902:3903], cache[:, :, 3903:]
+    for Tq in (2, 150):
+        q, _, _, table, do = make(10, torch.bfloat16, B, Tq, 1, 1, 1, D, 32)
+        check_all(lib, q, k, v, table, do, (32, 128), offset=T - Tq)
+
+
+def test_other_streams_and_graph_replays(lib):
+    """side stream; a captured forward + backward replayed on new inputs with eager work between the replays, and two captured
+    graphs in turn: every replay equals the eager result bit for bit"""
+    ops, ob = lib
+    buckets = (32, 128)
+
+    def work(x):
+        out, lse = ops.mha_relbias(*x[:4], buckets, want_lse=True)
+        step = ops.mha_relbias(x[0][:, -1:], *x[1:4], buckets, offset=x[1].shape[1] - 1)
+        return (out, lse, step, *ob.mha_relbias_bwd(*x[:4], out, lse, x[4], buckets))
+
+    shapes = ((2, 150, 150, 4, 2, 64), (1, 130, 1500, 2, 1, 128))
+    graphs = []
+    for n, sh in enumerate(shapes):
+        x = list(make(20 + n, torch.bfloat16, *sh, 32))
+        want = work(x)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = work(x)
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = work(x)
+        graphs.append((g, x, y, sh))
+    for turn in range(3):
+        for n, (g, x, y, sh) in enumerate(graphs):
+            for a, b in zip(x, make(40 + 2 * turn + n, torch.bfloat16, *sh, 32)):
+                a.copy_(b)
+            g.replay()
+            eager = work(x)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(y, eager)), (turn, n)
+
+
+def test_first_use_under_capture_is_refused(lib):
+    ops, _ = lib
+    q, k, v, table, _ = make(11, torch.bfloat16, 1, 8, 8, 2, 2, 64, 32)
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="capture"):
+        with torch.cuda.graph(g):
+            ops.mha_relbias(q, k, v, table, (32, 97))
+    torch.cuda.synchronize()
+    ops.mha_relbias(q, k, v, table, (32, 97))
+
+
+def test_autograd_layer(lib):
+    """a layer as a user writes it - packed projection, padded batch, bias table, output projection - trained through autograd:
+    gradients of all parameters against float64 autograd of the formulas.  Tolerance: operands, out and the gradients between the
+    operators are bf16, about eight roundings of 2^-8 in a row, each independent over the elements and at most u / sqrt(3) on
+    average: 8^0.5 2^-8 / 3^0.5 = 6.4e-3 in the 2-norm, doubled."""
+    from css_amd.autograd import mha_relbias
+    torch.manual_seed(5)
+    B, T, H, Hk, D, M = 3, 90, 4, 2, 32, 96
+    lens = torch.tensor([90, 41, 64], dtype=torch.int32, device=DEV)
+    w1 = (torch.randn((H + 2 * Hk) * D, M, device=DEV) / M ** 0.5).requires_grad_()
+    w2 = (torch.randn(M, H * D, device=DEV) / (H * D) ** 0.5).requires_grad_()
+    table = torch.randn(32, H, device=DEV, requires_grad=True)
+    x = torch.randn(B, T, M, device=DEV)
+    up = torch.randn(B, T, M, device=DEV)
+    inside = (torch.arange(T, device=DEV)[None] < lens[:, None])[..., None]
+
+    def layer(x, w1, w2, table, attend):
+        p = x @ w1.t()
+        q, k, v = p.split((H * D, Hk * D, Hk * D), -1)
+        o = attend(q.view(B, T, H, D), k.view(B, T, Hk, D), v.view(B, T, Hk, D), table)
+        return ((o.reshape(B, T, H * D) @ w2.t()) * up.to(x.dtype) * inside).sum()
+
+    def ours(q, k, v, table):
+        return mha_relbias(q.bfloat16(), k.bfloat16(), v.bfloat16(), table, (32, 128), k_lens=lens, q_lens=lens).to(q.dtype)
+
+    def plain(q, k, v, table):
+        r = torch.arange(T)[None] - torch.arange(T)[:, None]
+        place = torch.tensor([bucket(32, 128, True, x) for x in range(-T + 1, T)])[r + T - 1].to(DEV)
+        kk, vv = (y.repeat_interleave(H // Hk, 2).transpose(1, 2) for y in (k, v))
+        s = (q.transpose(1, 2) @ kk.transpose(2, 3).contiguous()) * D ** -0.5 + table[place].permute(2, 0, 1)
+        s = s.masked_fill(~inside[:, None, None, :, 0], -math.inf)
+        return (torch.softmax(s, -1) @ vv).transpose(1, 2) * inside[..., None]
+
+    layer(x, w1, w2, table, ours).backward()
+    got = [t.grad.clone() for t in (w1, w2, table)]
+    d = [t.detach().double().requires_grad_() for t in (w1, w2, table)]
+    layer(x.double(), *d, plain).backward()
+    for a, b in zip(got, d):
+        assert float((a.double() - b.grad).norm() / b.grad.norm()) < 2 * 6.4e-3
+    # differences: along the gradient the loss moves as its square says (float64 formulas at both ends)
+    with torch.no_grad():
+        h, ends = 1e-4, []
+        for sign in (1, -1):
+            moved = [t.detach().double() + sign * h * g.double() / g.double().norm() for t, g in zip((w1, w2, table), got)]
+            ends.append(float(layer(x.double(), *moved, plain)))
+        slope = (ends[0] - ends[1]) / (2 * h)
+        want = sum(float(g.double().norm()) for g in got)
+        assert abs(slope - want) < 2e-2 * want
+    q = torch.randn(1, 4, 2, 32, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    y = mha_relbias(q, q, q, table[:, :2], (32, 128))
+    g, = torch.autograd.grad(y.float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):  # no second derivative
+        g.sum().backward()
+
+
+def test_broadcast_gradient_and_shared_heads(lib):
+    """an expanded (stride 0) upstream gradient and values expanded over the batch: gradients land on the one copy"""
+    from css_amd.autograd import mha_relbias
+    torch.manual_seed(6)
+    q = torch.randn(4, 50, 4, 32, device=DEV).bfloat16().requires_grad_()
+    k = torch.randn(4, 50, 1, 32, device=DEV).bfloat16().requires_grad_()
+    v1 = torch.randn(1, 50, 1, 32, device=DEV).bfloat16().requires_grad_()
+    table = torch.randn(16, 4, device=DEV, requires_grad=True)
+    y = mha_relbias(q, k, v1.expand(4, -1, -1, -1), table, (16, 40))
+    y.sum().backward()
+    ref, mag = reference(q, k, v1.expand(4, -1, -1, -1), table, (16, 40), dout=torch.ones_like(y), out=y)
+    want, m = ref["dv"].sum(0, keepdim=True), mag["dv"].sum(0, keepdim=True)
+    # four rounded gradients are added in bf16: three more roundings
+    assert ((v1.grad.cpu().double() - want).abs() <= 4 * 2.0 ** -8 * m + 1e-6).all()
+    within("dk", k.grad, ref["dk"], mag["dk"], torch.bfloat16, 200, 1.0)
+
+
 def test_refusals(lib):
     ops, ob = lib
     q, k, v, table, do = make(7, torch.bfloat16, 2, 8, 8, 4, 2, 64, 32)
