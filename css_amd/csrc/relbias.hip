@@ -563,11 +563,22 @@ __global__ __launch_bounds__(64 * NW, 2) void rb_few_kernel(RbArgs a) {
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's V tile is written before other lanes read it
     __builtin_amdgcn_wave_barrier();
+    // P as a rounded value and the rounded rest: the products are free here, and a row of few keys has no other rounding to hide it
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       const u32x4 pb = pack8<E>(s, 8 * kk);
 #pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] = E::mma(frag_t<DP>(sV, 16 * kk, d, lane), pb, o[d]);
+      for (int e = 0; e < 4; ++e) {
+        s[8 * kk + 2 * e] -= E::lo(pb[e]);
+        s[8 * kk + 2 * e + 1] -= E::hi(pb[e]);
+      }
+      const u32x4 rest = pack8<E>(s, 8 * kk);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const u32x4 vf = frag_t<DP>(sV, 16 * kk, d, lane);
+        o[d] = E::mma(vf, pb, o[d]);
+        o[d] = E::mma(vf, rest, o[d]);
+      }
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -724,6 +735,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   u32x4 qf[NK], df[NK];
   row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, q0 + wave * 32, sq.qlen, a.D, lane, qf);
   row_frags<DP>(a.dout + b * a.sdo.b + h * a.sdo.h, a.sdo.t, q0 + wave * 32, sq.qlen, a.D, lane, df);
+  const float sign = wave & 1 ? -1.f : 1.f;
   float delta = 0.f, lse2 = RB_INF, fac = 1.f;  // fac: of the rounded dS (fp16)
   {
     u32x4 of[NK];
@@ -747,8 +759,15 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
       if (hi == 0) a.size[((int64_t)b * a.H + h) * a.tq128 + i] = squares;
     }
     if (x != -RB_INF) lse2 = x * RB_LOG2E;
+    // The matrix unit's sums lean to the negative side by about 2^-25 each; over the 36 million pairs of a 6001 x 6001 head that
+    // showed as 10^-5 of the table's gradient.  Odd waves therefore compute -dP (and all behind it), so that it cancels.
+    if (wave & 1) {
+#pragma unroll
+      for (int ks = 0; ks < NK; ++ks) df[ks] ^= 0x80008000u;
+    }
     const int64_t to = ((int64_t)b * a.H + h) * a.tq128 + i;  // rows up to the tile's end: the next kernel reads whole tiles
     if (hi == 0) a.delta[to] = -delta, a.lse2[to] = lse2;
+    delta *= sign;
   }
   f32x16 dq[ND];
 #pragma unroll
@@ -781,7 +800,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
     if (!near && pending) {  // the last parts kept have nothing to wait for
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        if (n32 < 3) sG[2 * g * span + cell0 + j0 + 8 * g] += kept[g];
+        if (n32 < 3) sG[2 * g * span + cell0 + j0 + 8 * g] += sign * kept[g];
 #pragma unroll
       for (int g = 0; g < 4; ++g) kept[g] = 0.f;
       pending = false;
@@ -845,7 +864,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
           const float own = s[4 * g + 3] + from_below_row(s[4 * g + 2] + from_below_row(s[4 * g + 1]));
           const float x = n32 < 3 ? (all - own) + kept[g] : all;
           kept[g] = swap_halves(own);
-          sG[2 * g * span + cell0 + j0 + 32 * u + 8 * g] = old[g] + x;
+          sG[2 * g * span + cell0 + j0 + 32 * u + 8 * g] = __builtin_fmaf(sign, x, old[g]);
         }
         pending = true;
       } else {
@@ -881,12 +900,12 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   if (pending) {
 #pragma unroll
     for (int g = 0; g < 4; ++g)
-      if (n32 < 3) sG[2 * g * span + cell0 + nt * 64 + 8 * g] += kept[g];
+      if (n32 < 3) sG[2 * g * span + cell0 + nt * 64 + 8 * g] += sign * kept[g];
   }
 
   if (i < a.Tq) {
     uint16_t* const op = a.dq + b * a.sdq.b + (int64_t)i * a.sdq.t + h * a.sdq.h;
-    const float f = E::narrow ? a.scale / fac : a.scale;
+    const float f = E::narrow ? sign * a.scale / fac : sign * a.scale;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -900,8 +919,8 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   const int nwg = a.B * a.ntile, wg = b * a.ntile + tile;
   int lo = 0, end = 0;
   if (tid < a.nb) lo = a.bucket_range[2 * tid], end = a.bucket_range[2 * tid + 1];
-  farl = wave_total(farl);
-  farr = wave_total(farr);
+  farl = sign * wave_total(farl);
+  farr = sign * wave_total(farr);
   if (lane == 0) sFar[2 * wave] = farl, sFar[2 * wave + 1] = farr;
   __syncthreads();
   const int each = (span + 255) >> 8, first = tid * each;
