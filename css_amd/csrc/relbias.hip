@@ -123,9 +123,12 @@ DEV int xcd_order(int id, int n) {
   return x * full + min(x, rest) + i;
 }
 
-// Causal rows: the last tiles are the longest, and start first.  Every second 256 workgroups the order turns round: a CU that took a
-// long one of the first 256 gets a short one of the next (both sit on it at once).
-DEV int row_tile(const RbArgs& a, int rank) { return a.causal && ((blockIdx.x >> 8) & 1) ? rank : a.ntile - 1 - rank; }
+// Causal rows: the last tiles are the longest, and start first.  A CU that takes one of an XCD's first 32 workgroups gets one of its
+// next 32 as well, and both sit on it at once: the order turns round with the heads that fill 32 workgroups, so that a long one
+// meets a short one.  (The turn has to be the same for all tiles of a head: each tile is taken once.)
+DEV int row_tile(const RbArgs& a, int head, int rank) {
+  return a.causal && ((head * a.ntile) >> 5 & 1) ? rank : a.ntile - 1 - rank;
+}
 
 // table entry -> score units (the products' accumulators hold q . k, scaled later by c2)
 DEV float bias_units(const RbArgs& a, float w) { return w <= -RB_BIG ? -RB_INF : (w > RB_BIG ? RB_BIG : w) * a.inv_scale; }
@@ -292,7 +295,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const int id = xcd_order(blockIdx.x, a.nblk);
   const Quot it = split(id, a.per_tile), bh = split(it.q, a.per_head);
-  const int b = bh.q, h = bh.r, hk = a.per_group.over(h), tile = row_tile(a, it.r);
+  const int b = bh.q, h = bh.r, hk = a.per_group.over(h), tile = row_tile(a, it.q, it.r);
   const Seq sq = seq_of(a, b);
   const int q0 = tile * 128, i = q0 + wave * 32 + n32, p0 = sq.off + q0 + wave * 32;
   int kend = q0 < sq.qlen ? sq.klen : 0, wend = q0 + wave * 32 < sq.qlen ? sq.klen : 0;
@@ -714,7 +717,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const int id = xcd_order(blockIdx.x, a.nblk);
   const Quot it = split(id, a.per_tile), bh = split(it.q, a.per_head);
-  const int b = bh.q, h = bh.r, hk = a.per_group.over(h), tile = row_tile(a, it.r);
+  const int b = bh.q, h = bh.r, hk = a.per_group.over(h), tile = row_tile(a, it.q, it.r);
   const Seq sq = seq_of(a, b);
   const int q0 = tile * 128, i = q0 + wave * 32 + n32, p0 = sq.off + q0 + wave * 32;
   int kend = q0 < sq.qlen ? sq.klen : 0, wend = q0 + wave * 32 < sq.qlen ? sq.klen : 0;

@@ -257,6 +257,16 @@ def test_same_bits_every_time(lib):
         assert all(torch.equal(a, b) for a, b in zip(first, got))
 
 
+@pytest.mark.parametrize("B,H,Hk,Tq,Tk,causal", [(8, 10, 5, 520, 520, True), (7, 11, 11, 300, 390, True), (9, 12, 4, 270, 270, False),
+                                                (1, 3, 3, 1400, 1400, True)])
+def test_many_workgroups(lib, B, H, Hk, Tq, Tk, causal):
+    """hundreds of workgroups whose heads do not fall on the 256 or 32 of one round of the chip: every tile is taken, and once"""
+    q, k, v, table, do = make(12, torch.bfloat16, B, Tq, Tk, H, Hk, 32, 32)
+    stale = [torch.full((n,), float("nan"), device="cuda") for n in [1 << 24] * 4 + [1 << 17] * 16]     # what a tile left out shows
+    del stale
+    check_all(lib, q, k, v, table, do, (32, 128), causal=causal, offset=Tk - Tq)
+
+
 def test_small_gradients_in_fp16(lib):
     """dS has the size of the incoming gradient: 2^-14 here, and a thousandth of that per key.  Rounded as it is, dS would lie among
     fp16's subnormals (relative error 10^-2 and more); roundings to full precision are independent, u / sqrt(3) each at most
