@@ -127,7 +127,7 @@ DEV int xcd_order(int id, int n) {
 // next 32 as well, and both sit on it at once: the order turns round with the heads that fill 32 workgroups, so that a long one
 // meets a short one.  (The turn has to be the same for all tiles of a head: each tile is taken once.)
 DEV int row_tile(const RbArgs& a, int head, int rank) {
-  return a.causal && ((head * a.ntile) >> 5 & 1) ? rank : a.ntile - 1 - rank;
+  return a.causal && ((head * a.ntile * a.nsplit) >> 5 & 1) ? rank : a.ntile - 1 - rank;
 }
 
 // table entry -> score units (the products' accumulators hold q . k, scaled later by c2)
@@ -702,6 +702,7 @@ DEV float swap_halves(float x) {
 
 // dq and the table's gradient: 4 waves x 32 queries of one (sequence, head) against 64-key tiles.
 //   S^T = K Q^T (+ bias), dP^T = V dO^T (from -delta), dS = P dP, dQ^T += K^T dS^T
+// Where few workgroups would run, the keys are split over `nsplit` of them, whose sums rb_dq_join_kernel adds in order.
 // It also leaves delta_i = do_i . o_i and the rows' log-sum-exp in log2 units for the next kernel, +inf where a row has no
 // keys or lies behind its sequence (exp2(s - inf) = 0: such rows drop out of every product).
 template <class E, int DP>
@@ -716,8 +717,8 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   double* const sFar = reinterpret_cast<double*>(smem + 4 * TILE + ((9 * span + 1) / 2 * 2) * 4);  // [4][2], [4]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const int id = xcd_order(blockIdx.x, a.nblk);
-  const Quot it = split(id, a.per_tile), bh = split(it.q, a.per_head);
-  const int b = bh.q, h = bh.r, hk = a.per_group.over(h), tile = row_tile(a, it.q, it.r);
+  const Quot is = split(id, a.per_split), it = split(is.q, a.per_tile), bh = split(it.q, a.per_head);
+  const int part = is.r, b = bh.q, h = bh.r, hk = a.per_group.over(h), tile = row_tile(a, it.q, it.r);
   const Seq sq = seq_of(a, b);
   const int q0 = tile * 128, i = q0 + wave * 32 + n32, p0 = sq.off + q0 + wave * 32;
   int kend = q0 < sq.qlen ? sq.klen : 0, wend = q0 + wave * 32 < sq.qlen ? sq.klen : 0;
@@ -725,13 +726,14 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
     kend = min(kend, sq.off + min(q0 + 128, sq.qlen));
     wend = min(wend, p0 + 32);
   }
-  const int nt = kend > 0 ? (kend + 63) >> 6 : 0;
+  const int tiles = kend > 0 ? (kend + 63) >> 6 : 0;
+  const int ta = a.per_split.over(tiles * part), nt = a.per_split.over(tiles * (part + 1));  // this workgroup's key tiles
 
   TileDma<DP> dK, dV;
-  dK.init(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, 0, sq.klen, a.D, wave, lane);
-  dV.init(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, 0, sq.klen, a.D, wave, lane);
+  dK.init(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, ta, sq.klen, a.D, wave, lane);
+  dV.init(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, ta, sq.klen, a.D, wave, lane);
   const unsigned lK = lds_addr(sK), lV = lds_addr(sV);
-  if (nt > 0) {
+  if (ta < nt) {
     dK.next(lK, wave);
     dV.next(lV, wave);
   }
@@ -759,7 +761,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
         for (int e = 0; e < 4; ++e) squares += E::lo(df[ks][e]) * E::lo(df[ks][e]) + E::hi(df[ks][e]) * E::hi(df[ks][e]);
       squares = half_sum(squares);
       fac = row_factor(squares);
-      if (hi == 0) a.size[((int64_t)b * a.H + h) * a.tq128 + i] = squares;
+      if (hi == 0 && part == 0) a.size[((int64_t)b * a.H + h) * a.tq128 + i] = squares;
     }
     if (x != -RB_INF) lse2 = x * RB_LOG2E;
     // The matrix unit's sums lean to the negative side by about 2^-25 each; over the 36 million pairs of a 6001 x 6001 head that
@@ -769,7 +771,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
       for (int ks = 0; ks < NK; ++ks) df[ks] ^= 0x80008000u;
     }
     const int64_t to = ((int64_t)b * a.H + h) * a.tq128 + i;  // rows up to the tile's end: the next kernel reads whole tiles
-    if (hi == 0) a.delta[to] = -delta, a.lse2[to] = lse2;
+    if (hi == 0 && part == 0) a.delta[to] = -delta, a.lse2[to] = lse2;
     delta *= sign;
   }
   f32x16 dq[ND];
@@ -896,7 +898,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
     dma_wait();
     __syncthreads();
   };
-  for (int t = 0; t < nt; t += 2) {
+  for (int t = ta; t < nt; t += 2) {
     step(t, Const<0>{});
     if (t + 1 < nt) step(t + 1, Const<1>{});
   }
@@ -906,7 +908,16 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
       if (n32 < 3) sG[2 * g * span + cell0 + nt * 64 + 8 * g] += sign * kept[g];
   }
 
-  if (i < a.Tq) {
+  if (i < a.Tq && a.nsplit > 1) {  // sums in f32: [split][sequence, head, query][DP]
+    float* const pq = a.part2 + ((((int64_t)part * a.B + b) * a.H + h) * a.Tq + i) * DP;
+    const float f = E::narrow ? sign / fac : sign;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(pq + 32 * d + 8 * g + 4 * hi) =
+            f32x4{dq[d][4 * g] * f, dq[d][4 * g + 1] * f, dq[d][4 * g + 2] * f, dq[d][4 * g + 3] * f};
+  } else if (i < a.Tq) {
     uint16_t* const op = a.dq + b * a.sdq.b + (int64_t)i * a.sdq.t + h * a.sdq.h;
     const float f = E::narrow ? sign * a.scale / fac : sign * a.scale;
 #pragma unroll
@@ -919,7 +930,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   }
   // The workgroup's share of the table's gradient.  A bucket's distances are contiguous: running sums over the distances in 64
   // bits, and a bucket is the difference of two (one thread per bucket adding up its distances took 4 us).
-  const int nwg = a.B * a.ntile, wg = b * a.ntile + tile;
+  const int nwg = a.B * a.ntile * a.nsplit, wg = (b * a.ntile + tile) * a.nsplit + part;
   int lo = 0, end = 0;
   if (tid < a.nb) lo = a.bucket_range[2 * tid], end = a.bucket_range[2 * tid + 1];
   farl = sign * wave_total(farl);
@@ -1186,6 +1197,19 @@ __global__ __launch_bounds__(256) void rb_dkv_join_kernel(RbArgs a) {
   store4<E>((key ? a.dk : a.dv) + b * st.b + (int64_t)j * st.t + hk * st.h + c, y[0], y[1], y[2], y[3]);
 }
 
+// dq from the splits' sums, in order; a thread has 4 elements of one row
+template <class E, int DP>
+__global__ __launch_bounds__(256) void rb_dq_join_kernel(RbArgs a) {
+  const int64_t rows = (int64_t)a.B * a.H * a.Tq, x = (int64_t)blockIdx.x * 256 + threadIdx.x, row = x / (DP / 4);
+  const int c = (int)(x % (DP / 4)) * 4;
+  if (row >= rows || c >= a.D) return;
+  const int64_t bh = row / a.Tq;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.nsplit; ++s) y += *reinterpret_cast<const f32x4*>(a.part2 + ((int64_t)s * rows + row) * DP + c);
+  y *= a.scale;
+  store4<E>(a.dq + bh / a.H * a.sdq.b + row % a.Tq * a.sdq.t + bh % a.H * a.sdq.h + c, y[0], y[1], y[2], y[3]);
+}
+
 // =============================================================================================== host side
 bool strides_ok(const int64_t* s, int D) {
   // 16-byte rows that do not overlap; a tile of 64 rows must stay within a 31-bit byte offset
@@ -1238,10 +1262,11 @@ size_t dkv_lds(int DP, int md) { return fwd_lds(DP, md) + 1024 + 16; }
 // launches with more than 64 KB of LDS have to be allowed, per device: asked for at each such launch
 template <class K>
 int launch(K kernel, int64_t blocks, size_t lds, RbArgs a, int heads, hipStream_t s, int threads = 256) {
+  if (a.nsplit < 1) a.nsplit = 1;
   a.per_tile.set(a.ntile < 1 ? 1 : a.ntile);
   a.per_head.set(heads);
   a.per_group.set(a.H / a.Hk);
-  a.per_split.set(a.nsplit < 1 ? 1 : a.nsplit);
+  a.per_split.set(a.nsplit);
   if (lds > 64 * 1024 &&
       hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
     return CSSHIP_ELAUNCH;
@@ -1250,13 +1275,15 @@ int launch(K kernel, int64_t blocks, size_t lds, RbArgs a, int heads, hipStream_
   return CSSHIP_OK;
 }
 
-// Which forward: rb_fwd_kernel reuses a K / V tile for 128 queries, rb_few_kernel for 32 rows but may take all heads of a group at
-// once and split the keys.  The latter where the former would leave most of the chip idle.
+// Which forward: rb_fwd_kernel reuses a K / V tile for 128 queries, rb_few_kernel for 32 rows but takes all heads of a group at
+// once and may split the keys.  The latter from 256 keys on, where the former would leave most of the chip idle (4 heads of 64,
+// 256 x 1000: 12.2 us against 20.5; 2000 x 2000, 64 workgroups: 26.9 against 35.9) or most of its 128 rows empty (16 x 16 heads
+// in groups of 4, 20 x 2000: 22.4 against 33.3).  At 256 keys both take 8 us, at 64 the former 5 and the latter 6.7.
 struct FwdPlan { bool few; int ntile, nsplit; };
 FwdPlan fwd_plan(const csship_relbias* p) {
   const int64_t rows = (int64_t)p->Tq * (p->H / p->Hk), tiles = (rows + 31) / 32, wide = (int64_t)p->B * p->H * ((p->Tq + 127) / 128);
-  FwdPlan f{rows <= 32 || (wide < 128 && p->Tk >= 1024), (int)tiles, 1};
-  if (f.few && p->Tk > 1024) {  // 1024 keys and less: 8 tiles a wave, no second launch
+  FwdPlan f{p->Tk >= 256 && (p->Tq <= 32 || wide < 128), (int)tiles, 1};
+  if (f.few && p->Tk > 1024) {  // up to there no second launch pays: 4 x 8 heads, 256 x 1000: 14.2 us against 22.1 split at 256
     const int64_t want = 768 / ((int64_t)p->B * p->Hk * tiles), most = (p->Tk + 511) / 512;
     f.nsplit = (int)(want < 1 ? 1 : want < most ? want : most);
   }
@@ -1272,7 +1299,7 @@ int launch_fwd(RbArgs a, const csship_relbias* p, hipStream_t s) {
     a.nsplit = f.nsplit;
     a.nblk = a.B * a.Hk * a.ntile * a.nsplit;
     const int table = (a.H / a.Hk) * (2 * a.mde + 1), staged = table <= RB_FEW_TABLE ? table * 4 : 0;
-    // few workgroups: twice the waves, half the tiles for each (1 x 500 keys, 4 heads: FEWUS)
+    // few workgroups: twice the waves, half the tiles for each (1 x 500 keys, 4 heads: 8.5 us for 9.9)
     const int rc = a.nblk < 256 ? launch(rb_few_kernel<E, DP, 8>, a.nblk, few_area<DP, 8>() + staged, a, a.Hk, s, 512)
                                 : launch(rb_few_kernel<E, DP, 4>, a.nblk, few_area<DP, 4>() + staged, a, a.Hk, s);
     if (rc) return rc;
@@ -1290,17 +1317,31 @@ int launch_fwd(RbArgs a, const csship_relbias* p, hipStream_t s) {
 int dkv_splits(const csship_relbias* p) {
   const int64_t wgs = (int64_t)p->B * p->Hk * ((p->Tk + 127) / 128), steps = (int64_t)(p->H / p->Hk) * ((p->Tq + 63) / 64);
   if (wgs == 0) return 1;
-  const int64_t want = 512 / wgs, most = steps / 8 < 8 ? steps / 8 : 8;
+  const int64_t want = 512 / wgs, most = steps / 4 < 32 ? steps / 4 : 32;
+  return (int)(want < 1 || most < 1 ? 1 : want < most ? want : most);
+}
+
+// The same for the dq kernel's 128 queries and their keys (64 at a time), not below 4 steps.
+int dq_splits(const csship_relbias* p) {
+  const int64_t wgs = (int64_t)p->B * p->H * ((p->Tq + 127) / 128), steps = (p->Tk + 63) / 64;
+  if (wgs == 0) return 1;
+  const int64_t want = 768 / wgs, most = steps / 2 < 8 ? steps / 2 : 8;
   return (int)(want < 1 || most < 1 ? 1 : want < most ? want : most);
 }
 
 template <class E, int DP>
 int launch_bwd(RbArgs a, const csship_relbias* p, hipStream_t s) {
-  a.ntile = a.nqtile = (a.Tq + 127) / 128;
+  a.ntile = (a.Tq + 127) / 128;
   a.tq128 = a.ntile * 128;
-  a.nblk = a.B * a.H * a.ntile;
-  if (a.nblk > 0)
+  a.nsplit = dq_splits(p);
+  a.nqtile = a.ntile * a.nsplit;
+  a.nblk = a.B * a.H * a.nqtile;
+  if (a.nblk > 0) {
     if (const int rc = launch(rb_dq_kernel<E, DP>, a.nblk, dq_lds(DP, a.mde), a, a.H, s)) return rc;
+    if (a.nsplit > 1)
+      if (const int rc = launch(rb_dq_join_kernel<E, DP>, ((int64_t)a.B * a.H * a.Tq * (DP / 4) + 255) / 256, 0, a, a.H, s)) return rc;
+  }
+  // (part2 again: the dq kernel's sums have been joined)
   a.ntile = (a.Tk + 127) / 128;
   a.nsplit = dkv_splits(p);
   a.nblk = a.B * a.Hk * a.ntile * a.nsplit;
@@ -1322,7 +1363,9 @@ int bwd_by_width(const RbArgs& a, const csship_relbias* p, hipStream_t s) {
 int64_t row_words(const csship_relbias* p) { return (int64_t)p->B * p->H * ((p->Tq + 127) / 128 * 128); }
 
 // the table gradient's shares: one number per workgroup of the dq kernel and bucket, in whole 16 bytes
-int64_t part_words(const csship_relbias* p) { return ((int64_t)p->B * p->H * ((p->Tq + 127) / 128) * p->n_buckets + 3) / 4 * 4; }
+int64_t part_words(const csship_relbias* p) {
+  return ((int64_t)p->B * p->H * ((p->Tq + 127) / 128) * dq_splits(p) * p->n_buckets + 3) / 4 * 4;
+}
 
 }  // namespace
 
@@ -1355,7 +1398,10 @@ int csship_relbias_fwd(const csship_relbias* p, uint16_t* out, const int64_t* ou
 size_t csship_relbias_bwd_workspace(const csship_relbias* p) {
   if (check_args(p) != CSSHIP_OK) return 0;
   const int splits = dkv_splits(p);
-  const int64_t sums = splits == 1 ? 0 : (int64_t)splits * 2 * p->B * p->Hk * p->Tk * width_of(p->D);
+  const int qsplits = dq_splits(p);
+  const int64_t sums_k = splits == 1 ? 0 : (int64_t)splits * 2 * p->B * p->Hk * p->Tk * width_of(p->D);
+  const int64_t sums_q = qsplits == 1 ? 0 : (int64_t)qsplits * p->B * p->H * p->Tq * width_of(p->D);
+  const int64_t sums = sums_k > sums_q ? sums_k : sums_q;  // one after the other in the same memory
   return (size_t)(3 * row_words(p) + part_words(p) + sums) * 4 + 16;
 }
 
