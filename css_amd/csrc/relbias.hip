@@ -20,6 +20,7 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 
 constexpr float RB_LOG2E = 1.4426950408889634f, RB_LN2 = 0.6931471805599453f;
 constexpr int RB_PAD = 96;          // entries of the spread table beyond the largest distance on each side: a 64 x 32 tile that
@@ -235,20 +236,31 @@ DEV void row_frags(const uint16_t* base, int64_t st, int first, int rows, int D,
   }
 }
 
-// operand fragment of row r of a tile: the 16-byte piece 2 ks + hi
+// Where a lane reads its operand fragments in a tile: two addresses, the others differ from them in piece bits (an exclusive or)
+// and by constants.
 template <int DP>
-DEV u32x4 frag(const unsigned char* tile, int r, int ks, int hi) {
-  return *reinterpret_cast<const u32x4*>(tile + tile_at<DP>(r, 2 * ks + hi));
-}
-// transposed fragment: rows (= reduction index) kb + 4 hi + 0..3 and kb + 8 + 4 hi + 0..3, column 32 dt + (lane & 31)
-template <int DP>
-DEV u32x4 frag_t(const unsigned char* tile, int kb, int dt, int lane) {
-  const int l16 = lane & 15, hi = lane >> 5;
-  const int r0 = kb + 4 * hi + (l16 >> 2), c = 4 * dt + ((lane >> 4) & 1) * 2 + ((l16 & 3) >> 1), by = (l16 & 1) * 8;
-  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + tile_at<DP>(r0, c) + by));
-  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + tile_at<DP>(r0 + 8, c) + by));
-  return __builtin_bit_cast(u32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-}
+struct LaneAt {
+  static constexpr unsigned P = 2 * DP;
+  unsigned row, tr;
+  __device__ __forceinline__ explicit LaneAt(int lane) {
+    const int l16 = lane & 15, hi = lane >> 5;
+    row = tile_at<DP>(lane & 31, hi);
+    tr = tile_at<DP>(4 * hi + (l16 >> 2), ((lane >> 4) & 1) * 2 + ((l16 & 3) >> 1)) + (l16 & 1) * 8;
+  }
+  // Makes the compiler derive the other addresses here: held over the loop they do not fit the registers beside 128 columns, and
+  // a reload from scratch waits for the tiles under way as well.
+  __device__ __forceinline__ void renew() { asm volatile("" : "+v"(row), "+v"(tr)); }
+  // row first + (lane & 31), piece 2 ks + hi; first: a multiple of 32
+  __device__ __forceinline__ u32x4 frag(unsigned tile, int first, int ks) const {
+    return *(const lds_u32x4*)(uintptr_t)((row ^ (ks << 5)) + (tile + first * P));
+  }
+  // transposed: rows (= reduction index) kb + 4 hi + 0..3 and kb + 8 + 4 hi + 0..3, column 32 dt + (lane & 31); kb: a multiple of 16
+  __device__ __forceinline__ u32x4 frag_t(unsigned tile, int kb, int dt) const {
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)((tr ^ (dt << 6)) + (tile + kb * P)));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)((tr ^ (dt << 6 | 32)) + (tile + (kb + 8) * P)));
+    return __builtin_bit_cast(u32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
 
 template <class E>
 DEV u32x4 pack8(const f32x16& s, int first) {
@@ -309,6 +321,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
   dk.init(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, 0, sq.klen, a.D, wave, lane);
   dv.init(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, 0, sq.klen, a.D, wave, lane);
   const unsigned lK = lds_addr(sK), lV = lds_addr(sV);
+  const LaneAt<DP> at(lane);
   if (nt > 0) {
     dk.next(lK, wave);
     dv.next(lV, wave);
@@ -335,8 +348,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
       dv.next(lV + (buf ^ 1) * TILE, wave);
     };
     if (j0 < wend) {
-      const unsigned char* const kt = sK + buf * TILE;
-      const unsigned char* const vt = sV + buf * TILE;
+      const unsigned kt = lK + buf * TILE, vt = lV + buf * TILE;
       f32x16 s[2];
       // S^T = K Q^T + bias.  Operands are requested in groups ahead of the products that use them: left alone, the compiler
       // reads, waits and multiplies one fragment at a time.
@@ -348,7 +360,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
 #pragma unroll
           for (int ks = 0; ks < GK && k0 + ks < NK; ++ks)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) kf[ks][u] = frag<DP>(kt, 32 * u + n32, k0 + ks, hi);
+            for (int u = 0; u < 2; ++u) kf[ks][u] = at.frag(kt, 32 * u, k0 + ks);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int ks = 0; ks < GK && k0 + ks < NK; ++ks)
@@ -374,7 +386,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) vf[kk][d] = frag_t<DP>(vt, 16 * kk, d, lane);
+        for (int d = 0; d < ND; ++d) vf[kk][d] = at.frag_t(vt, 16 * kk, d);
       __builtin_amdgcn_sched_barrier(0);
       if (j0 + 64 > sq.klen || (a.causal && j0 + 63 > p0)) {
         const int lim = (a.causal ? min(sq.klen, p0 + n32 + 1) : sq.klen) - j0 - 4 * hi;
@@ -419,7 +431,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) vg[kk][d] = frag_t<DP>(vt, 32 + 16 * kk, d, lane);
+        for (int d = 0; d < ND; ++d) vg[kk][d] = at.frag_t(vt, 32 + 16 * kk, d);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
@@ -459,6 +471,8 @@ __global__ __launch_bounds__(64 * NW, 2) void rb_few_kernel(RbArgs a) {
   constexpr int P = 2 * DP, NK = DP / 16, ND = DP / 32, CPR = DP / 8, RPI = 64 / CPR, NV = 32 / RPI, NT = 64 * NW;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   unsigned char* const sV = smem + wave * 32 * P;
+  const unsigned lV = lds_addr(sV);
+  const LaneAt<DP> at(lane);
   float* const sT = reinterpret_cast<float*>(smem + few_area<DP, NW>());
   const int G = a.per_group.d, R = a.Tq * G;
   const int id = xcd_order(blockIdx.x, a.nblk);
@@ -578,7 +592,7 @@ __global__ __launch_bounds__(64 * NW, 2) void rb_few_kernel(RbArgs a) {
       const u32x4 rest = pack8<E>(s, 8 * kk);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        const u32x4 vf = frag_t<DP>(sV, 16 * kk, d, lane);
+        const u32x4 vf = at.frag_t(lV, 16 * kk, d);
         o[d] = E::mma(vf, pb, o[d]);
         o[d] = E::mma(vf, rest, o[d]);
       }
@@ -733,6 +747,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   dK.init(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, ta, sq.klen, a.D, wave, lane);
   dV.init(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, ta, sq.klen, a.D, wave, lane);
   const unsigned lK = lds_addr(sK), lV = lds_addr(sV);
+  LaneAt<DP> at(lane);
   if (ta < nt) {
     dK.next(lK, wave);
     dV.next(lV, wave);
@@ -796,8 +811,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
       dV.next(lV + (buf ^ 1) * TILE, wave);
     };
     if (!(j0 < wend)) transfer();
-    const unsigned char* const kt = sK + buf * TILE;
-    const unsigned char* const vt = sV + buf * TILE;
+    const unsigned kt = lK + buf * TILE, vt = lV + buf * TILE;
     const bool active = j0 < wend;
     const bool near = active && j0 - (p0 + 31) < a.mde && j0 + 63 - p0 > -a.mde;
     const int pw = sq.off + q0;
@@ -817,6 +831,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
     for (int u = 0; u < 2; ++u) {
       if (u == 1 && any_near) __syncthreads();
       if (!active) continue;
+      if (DP == 128) at.renew();
       f32x16 s, dp = splat16(-delta);
       // operands in groups ahead of the products that use them, as in rb_fwd_kernel
       auto scores = [&](auto zero) {
@@ -826,8 +841,8 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
         for (int c = 0; c < NK; c += GK) {
 #pragma unroll
           for (int ks = 0; ks < GK && c + ks < NK; ++ks) {
-            kf[ks] = frag<DP>(kt, 32 * u + n32, c + ks, hi);
-            vf[ks] = frag<DP>(vt, 32 * u + n32, c + ks, hi);
+            kf[ks] = at.frag(kt, 32 * u, c + ks);
+            vf[ks] = at.frag(vt, 32 * u, c + ks);
           }
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -850,7 +865,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
 #pragma unroll
       for (int kk = 0; kk < (DP == 128 ? 0 : 2); ++kk)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) kf[kk][d] = frag_t<DP>(kt, 32 * u + 16 * kk, d, lane);
+        for (int d = 0; d < ND; ++d) kf[kk][d] = at.frag_t(kt, 32 * u + 16 * kk, d);
       __builtin_amdgcn_sched_barrier(0);
       if (edge) {
 #pragma unroll
@@ -889,7 +904,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
         const u32x4 ds = pack8<E>(s, 8 * kk);
         if (DP == 128) {  // (no registers to hold them across the exponentials)
 #pragma unroll
-          for (int d = 0; d < ND; ++d) kf[kk][d] = frag_t<DP>(kt, 32 * u + 16 * kk, d, lane);
+          for (int d = 0; d < ND; ++d) kf[kk][d] = at.frag_t(kt, 32 * u + 16 * kk, d);
         }
 #pragma unroll
         for (int d = 0; d < ND; ++d) dq[d] = E::mma(kf[kk][d], ds, dq[d]);
@@ -1021,6 +1036,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
   const int per = k0 < sq.klen ? max(((sq.qlen + 63) >> 6) - t0, 0) : 0, steps = per * G;
   const int it0 = (int)((int64_t)steps * part / a.nsplit), it1 = (int)((int64_t)steps * (part + 1) / a.nsplit);
   const unsigned lQ = lds_addr(sQ), lO = lds_addr(sO);
+  const LaneAt<DP> at(lane);
   float lrow = 0.f, fac = 2e37f;  // fac (fp16): above every factor until a gradient has been seen
 
   for (int it = it0; it < it1;) {
@@ -1055,8 +1071,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
       constexpr int buf = decltype(parity)::value;
       const bool more = t + 1 < tb;
       if (more) load(t + 1, buf ^ 1);
-      const unsigned char* const qt = sQ + buf * TILE;
-      const unsigned char* const ot = sO + buf * TILE;
+      const unsigned qt = lQ + buf * TILE, ot = lO + buf * TILE;
       const float* const lt = sL + buf * 128;
       if constexpr (E::narrow) {  // one factor for all of dK's sum so far: a tile of larger gradients takes it down
         const float top = sF[buf], f = row_factor(top);
@@ -1081,24 +1096,24 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] = bp[-(8 * (r >> 2) + (r & 3))];
         }
-        auto product = [&](const unsigned char* tile, const u32x4 (&f)[NK], f32x16& x) {  // x += rows of the tile . f
+        auto product = [&](unsigned tile, const u32x4 (&f)[NK], f32x16& x) {  // x += rows of the tile . f
           constexpr int GK = 4;
           u32x4 af[GK];
 #pragma unroll
           for (int c = 0; c < NK; c += GK) {
 #pragma unroll
-            for (int ks = 0; ks < GK && c + ks < NK; ++ks) af[ks] = frag<DP>(tile, 32 * u + n32, c + ks, hi);
+            for (int ks = 0; ks < GK && c + ks < NK; ++ks) af[ks] = at.frag(tile, 32 * u, c + ks);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int ks = 0; ks < GK && c + ks < NK; ++ks) x = E::mma(af[ks], f[c + ks], x);
           }
         };
-        auto outer = [&](const unsigned char* tile, const f32x16& x, f32x16 (&sum)[ND]) {  // sum += tile^T . x, x rounded here
+        auto outer = [&](unsigned tile, const f32x16& x, f32x16 (&sum)[ND]) {  // sum += tile^T . x, x rounded here
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) {
             u32x4 af[ND];
 #pragma unroll
-            for (int d = 0; d < ND; ++d) af[d] = frag_t<DP>(tile, 32 * u + 16 * kk, d, lane);
+            for (int d = 0; d < ND; ++d) af[d] = at.frag_t(tile, 32 * u + 16 * kk, d);
             const u32x4 xb = pack8<E>(x, 8 * kk);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
