@@ -124,11 +124,17 @@ DEV int xcd_order(int id, int n) {
   return x * full + min(x, rest) + i;
 }
 
-// Causal rows: the last tiles are the longest, and start first.  A CU that takes one of an XCD's first 32 workgroups gets one of its
-// next 32 as well, and both sit on it at once: the order turns round with the heads that fill 32 workgroups, so that a long one
-// meets a short one.  (The turn has to be the same for all tiles of a head: each tile is taken once.)
-DEV int row_tile(const RbArgs& a, int head, int rank) {
-  return a.causal && ((head * a.ntile * a.nsplit) >> 5 & 1) ? rank : a.ntile - 1 - rank;
+// The tile and key or query range of a workgroup.  Under `causal` tiles differ in length and the longest come first.  A CU that
+// takes one of an XCD's first 32 workgroups gets one of its next 32 as well, and both sit on it at once: every second 32 are
+// taken in reverse, within each head, so that a long one meets a short one (2 x 2047, 16 heads: forward 66 -> 55 us).
+struct Place { int head, rank, part; };  // (sequence, head); tile counted from the longest
+DEV Place place_of(const RbArgs& a) {
+  const int n = a.nblk, x = blockIdx.x & 7, i = blockIdx.x >> 3, id = xcd_order(blockIdx.x, n), base = id - i;
+  const int head = a.per_tile.over(a.per_split.over(id)), first = head * a.ntile * a.nsplit, last = first + a.ntile * a.nsplit;
+  int r = id;
+  if (a.causal && (i & 32)) r = max(first, base + (i & ~31)) + min(last, base + min((i | 31) + 1, (n >> 3) + (x < (n & 7)))) - 1 - id;
+  const Quot q = split(r - first, a.per_split);
+  return Place{head, q.q, q.r};
 }
 
 // table entry -> score units (the products' accumulators hold q . k, scaled later by c2)
@@ -183,21 +189,21 @@ DEV double wave_total(double x) {
   return x;
 }
 
-// ---- 64-row tiles of a [T, heads, D] tensor, memory -> LDS without passing registers (buffer_load_dwordx4 ... lds): one
+// ---- tiles of ROWS rows of a [T, heads, D] tensor, memory -> LDS without passing registers (buffer_load_dwordx4 ... lds): one
 // instruction of a wave fills 1 KB in lane order, so the swizzle is applied to the address each lane fetches.  Rows at or behind
 // `rows` and pieces at or behind D / 8 lie outside the descriptor: zeros.  Written as inline assembly because the compiler, which
 // cannot tell the double buffer's halves apart, otherwise waits for the transfer before every LDS read behind it; the
 // statement has no result registers, and dma_wait() stands before the barrier that hands the tile over.
-template <int DP>
+template <int DP, int ROWS = 64>
 struct TileDma {
-  static constexpr int CPR = DP / 8, RPI = 64 / CPR, N = 16 / RPI;  // pieces a row, rows an instruction, instructions a wave
+  static constexpr int CPR = DP / 8, RPI = 64 / CPR, N = ROWS / 4 / RPI;  // pieces a row, rows an instruction, instructions a wave
   unsigned off[N];
   uint64_t at;    // address of the next tile
   int64_t left;   // bytes from there to the end of the last row, 0 and less: none
-  unsigned step;  // bytes of 64 rows
+  unsigned step;  // bytes of ROWS rows
   __device__ __forceinline__ void init(const uint16_t* base, int64_t stride, int tile, int rows, int D, int wave, int lane) {
-    step = (unsigned)stride * 128u;
-    at = (uint64_t)(base + (int64_t)tile * 64 * stride);
+    step = (unsigned)stride * (2u * ROWS);
+    at = (uint64_t)(base + (int64_t)tile * ROWS * stride);
     left = rows > 0 ? ((int64_t)(rows - 1) * stride + D) * 2 - (int64_t)tile * step : 0;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -205,7 +211,7 @@ struct TileDma {
       off[n] = c * 8 < D ? (unsigned)r * (unsigned)stride * 2u + c * 16u : 0xfffffff0u;
     }
   }
-  // the next 64 rows to LDS byte address `lds`; all four waves take part
+  // the next ROWS rows to LDS byte address `lds`; all four waves take part
   __device__ __forceinline__ void next(unsigned lds, int wave) {
     const u32x4 rs = {(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((int)(at >> 32)) & 0xffffu,
                       (unsigned)__builtin_amdgcn_readfirstlane((int)(left <= 0 ? 0u : left < (int64_t)step ? (unsigned)left : step)), 0x00020000u};
@@ -305,9 +311,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
   unsigned char* const sV = smem + 2 * TILE;
   float* const sB = reinterpret_cast<float*>(smem + 4 * TILE);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
-  const int id = xcd_order(blockIdx.x, a.nblk);
-  const Quot it = split(id, a.per_tile), bh = split(it.q, a.per_head);
-  const int b = bh.q, h = bh.r, hk = a.per_group.over(h), tile = row_tile(a, it.q, it.r);
+  const Place at = place_of(a);
+  const Quot bh = split(at.head, a.per_head);
+  const int b = bh.q, h = bh.r, hk = a.per_group.over(h), tile = a.ntile - 1 - at.rank;
   const Seq sq = seq_of(a, b);
   const int q0 = tile * 128, i = q0 + wave * 32 + n32, p0 = sq.off + q0 + wave * 32;
   int kend = q0 < sq.qlen ? sq.klen : 0, wend = q0 + wave * 32 < sq.qlen ? sq.klen : 0;
@@ -321,7 +327,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
   dk.init(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, 0, sq.klen, a.D, wave, lane);
   dv.init(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, 0, sq.klen, a.D, wave, lane);
   const unsigned lK = lds_addr(sK), lV = lds_addr(sV);
-  const LaneAt<DP> at(lane);
+  const LaneAt<DP> in(lane);
   if (nt > 0) {
     dk.next(lK, wave);
     dv.next(lV, wave);
@@ -360,7 +366,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
 #pragma unroll
           for (int ks = 0; ks < GK && k0 + ks < NK; ++ks)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) kf[ks][u] = at.frag(kt, 32 * u, k0 + ks);
+            for (int u = 0; u < 2; ++u) kf[ks][u] = in.frag(kt, 32 * u, k0 + ks);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int ks = 0; ks < GK && k0 + ks < NK; ++ks)
@@ -386,7 +392,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) vf[kk][d] = at.frag_t(vt, 16 * kk, d);
+        for (int d = 0; d < ND; ++d) vf[kk][d] = in.frag_t(vt, 16 * kk, d);
       __builtin_amdgcn_sched_barrier(0);
       if (j0 + 64 > sq.klen || (a.causal && j0 + 63 > p0)) {
         const int lim = (a.causal ? min(sq.klen, p0 + n32 + 1) : sq.klen) - j0 - 4 * hi;
@@ -431,7 +437,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) vg[kk][d] = at.frag_t(vt, 32 + 16 * kk, d);
+        for (int d = 0; d < ND; ++d) vg[kk][d] = in.frag_t(vt, 32 + 16 * kk, d);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
@@ -730,9 +736,9 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   float* const sG = sB + span;                                      // [4 groups][2 halves][span]
   double* const sFar = reinterpret_cast<double*>(smem + 4 * TILE + ((9 * span + 1) / 2 * 2) * 4);  // [4][2], [4]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
-  const int id = xcd_order(blockIdx.x, a.nblk);
-  const Quot is = split(id, a.per_split), it = split(is.q, a.per_tile), bh = split(it.q, a.per_head);
-  const int part = is.r, b = bh.q, h = bh.r, hk = a.per_group.over(h), tile = row_tile(a, it.q, it.r);
+  const Place at = place_of(a);
+  const Quot bh = split(at.head, a.per_head);
+  const int part = at.part, b = bh.q, h = bh.r, hk = a.per_group.over(h), tile = a.ntile - 1 - at.rank;
   const Seq sq = seq_of(a, b);
   const int q0 = tile * 128, i = q0 + wave * 32 + n32, p0 = sq.off + q0 + wave * 32;
   int kend = q0 < sq.qlen ? sq.klen : 0, wend = q0 + wave * 32 < sq.qlen ? sq.klen : 0;
@@ -747,7 +753,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   dK.init(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, ta, sq.klen, a.D, wave, lane);
   dV.init(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, ta, sq.klen, a.D, wave, lane);
   const unsigned lK = lds_addr(sK), lV = lds_addr(sV);
-  LaneAt<DP> at(lane);
+  LaneAt<DP> in(lane);
   if (ta < nt) {
     dK.next(lK, wave);
     dV.next(lV, wave);
@@ -831,7 +837,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
     for (int u = 0; u < 2; ++u) {
       if (u == 1 && any_near) __syncthreads();
       if (!active) continue;
-      if (DP == 128) at.renew();
+      if (DP == 128) in.renew();
       f32x16 s, dp = splat16(-delta);
       // operands in groups ahead of the products that use them, as in rb_fwd_kernel
       auto scores = [&](auto zero) {
@@ -841,8 +847,8 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
         for (int c = 0; c < NK; c += GK) {
 #pragma unroll
           for (int ks = 0; ks < GK && c + ks < NK; ++ks) {
-            kf[ks] = at.frag(kt, 32 * u, c + ks);
-            vf[ks] = at.frag(vt, 32 * u, c + ks);
+            kf[ks] = in.frag(kt, 32 * u, c + ks);
+            vf[ks] = in.frag(vt, 32 * u, c + ks);
           }
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -865,7 +871,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
 #pragma unroll
       for (int kk = 0; kk < (DP == 128 ? 0 : 2); ++kk)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) kf[kk][d] = at.frag_t(kt, 32 * u + 16 * kk, d);
+        for (int d = 0; d < ND; ++d) kf[kk][d] = in.frag_t(kt, 32 * u + 16 * kk, d);
       __builtin_amdgcn_sched_barrier(0);
       if (edge) {
 #pragma unroll
@@ -904,7 +910,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
         const u32x4 ds = pack8<E>(s, 8 * kk);
         if (DP == 128) {  // (no registers to hold them across the exponentials)
 #pragma unroll
-          for (int d = 0; d < ND; ++d) kf[kk][d] = at.frag_t(kt, 32 * u + 16 * kk, d);
+          for (int d = 0; d < ND; ++d) kf[kk][d] = in.frag_t(kt, 32 * u + 16 * kk, d);
         }
 #pragma unroll
         for (int d = 0; d < ND; ++d) dq[d] = E::mma(kf[kk][d], ds, dq[d]);
@@ -1007,51 +1013,62 @@ DEV void table_sum(const RbArgs& a, int entry, int nwg) {
 // causal 2 x 2047 case).  Where few workgroups would run, the (head, query tile) steps are split over `nsplit`
 // workgroups, whose sums rb_dkv_join_kernel adds in order.
 template <class E, int DP>
-__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a) {
+__global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   if ((int)blockIdx.x >= a.nblk) {  // more table entries than waves (few keys)
     table_sum(a, blockIdx.x * 4 + (threadIdx.x >> 6), a.B * a.nqtile);
     return;
   }
-  constexpr int P = 2 * DP, TILE = 64 * P, NK = DP / 16, ND = DP / 32;
+  constexpr bool WIDE = DP == 128;
+  constexpr int ROWS = WIDE ? 32 : 64, P = 2 * DP, TILE = ROWS * P, NK = DP / 16, ND = DP / 32;
   unsigned char* const sQ = smem;
   unsigned char* const sO = smem + 2 * TILE;
-  float* const sL = reinterpret_cast<float*>(smem + 4 * TILE);  // [2][2][64] lse2 | -delta of a tile's rows
+  unsigned char* const sV = smem + 4 * TILE;  // [128 keys] of V (WIDE)
+  float* const sL = reinterpret_cast<float*>(sV + (WIDE ? 128 * P : 0));  // [2][2][64] lse2 | -delta of a tile's rows
   float* const sF = sL + 256;                                   // [2] largest sum of squares of a tile's rows of dout (fp16)
   float* const sB = sF + 4;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
-  const int id = xcd_order(blockIdx.x, a.nblk);
-  const Quot is = split(id, a.per_split), it_ = split(is.q, a.per_tile), bh = split(it_.q, a.per_head);
-  const int part = is.r, tile = it_.r, b = bh.q, hk = bh.r, G = a.per_group.d;
+  const Place at = place_of(a);
+  const Quot bh = split(at.head, a.per_head);
+  const int part = at.part, tile = at.rank, b = bh.q, hk = bh.r, G = a.per_group.d;
   const Seq sq = seq_of(a, b);
   const int k0 = tile * 128, j0 = k0 + wave * 32, j = j0 + n32;
-  u32x4 kf[NK], vf[NK];
+  u32x4 kf[NK], vf[WIDE ? 1 : NK];
   row_frags<DP>(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, j0, sq.klen, a.D, lane, kf);
-  row_frags<DP>(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, j0, sq.klen, a.D, lane, vf);
+  if constexpr (!WIDE) row_frags<DP>(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, j0, sq.klen, a.D, lane, vf);
   f32x16 dk[ND], dv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dk[d] = dv[d] = splat16(0.f);
   // causal: the first query that sees key k0 sits at position k0.  Steps are numbered head by head.
-  const int t0 = a.causal ? max(k0 - sq.off, 0) >> 6 : 0;
-  const int per = k0 < sq.klen ? max(((sq.qlen + 63) >> 6) - t0, 0) : 0, steps = per * G;
+  const int t0 = a.causal ? max(k0 - sq.off, 0) / ROWS : 0;
+  const int per = k0 < sq.klen ? max((sq.qlen + ROWS - 1) / ROWS - t0, 0) : 0, steps = per * G;
   const int it0 = (int)((int64_t)steps * part / a.nsplit), it1 = (int)((int64_t)steps * (part + 1) / a.nsplit);
   const unsigned lQ = lds_addr(sQ), lO = lds_addr(sO);
-  const LaneAt<DP> at(lane);
+  LaneAt<DP> in(lane);
+  const unsigned lV = lds_addr(sV) + wave * 32 * P;
+  if constexpr (WIDE) {
+    if (it0 < it1) {  // arrives with the first tile
+      TileDma<DP> dV;
+      dV.init(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, 2 * tile, sq.klen, a.D, wave, lane);
+      dV.next(lds_addr(sV), wave);
+      dV.next(lds_addr(sV) + 64 * P, wave);
+    }
+  }
   float lrow = 0.f, fac = 2e37f;  // fac (fp16): above every factor until a gradient has been seen
 
   for (int it = it0; it < it1;) {
     const int g = it / per, ta = t0 + it % per, tb = min(t0 + per, ta + it1 - it);  // one head's run of tiles
     it += tb - ta;
     const int h = hk * G + g;
-    TileDma<DP> dQ, dO;
+    TileDma<DP, ROWS> dQ, dO;
     dQ.init(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, ta, sq.qlen, a.D, wave, lane);
     dO.init(a.dout + b * a.sdo.b + h * a.sdo.h, a.sdo.t, ta, sq.qlen, a.D, wave, lane);
-    constexpr int ROWS = E::narrow ? 3 : 2;  // waves that bring a tile's row statistics
+    constexpr int STATS = E::narrow ? 3 : 2;  // waves that bring a tile's row statistics
     const float* const rl = (wave == 0 ? a.lse2 : wave == 1 ? a.delta : a.size) + ((int64_t)b * a.H + h) * a.tq128;
     auto load = [&](int t, int buf) {
       dQ.next(lQ + buf * TILE, wave);
       dO.next(lO + buf * TILE, wave);
-      if (wave < ROWS) lrow = rl[t * 64 + lane];
+      if (wave < STATS) lrow = rl[t * ROWS + (lane & (ROWS - 1))];
     };
     auto store = [&](int buf) {
       if (wave < 2) sL[buf * 128 + wave * 64 + lane] = lrow;
@@ -1085,9 +1102,10 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
         }
       }
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int p0 = sq.off + t * 64 + 32 * u;  // position of the sub-tile's first query
+      for (int u = 0; u < ROWS / 32; ++u) {
+        const int p0 = sq.off + t * ROWS + 32 * u;  // position of the sub-tile's first query
         if (j0 >= sq.klen || (a.causal && j0 > p0 + 31)) continue;
+        if (WIDE) in.renew();
         f32x16 s, dp;
         if (j0 - (p0 + 31) >= a.mde || j0 + 31 - p0 <= -a.mde) {
           s = splat16(j0 > p0 ? right : left);
@@ -1096,13 +1114,13 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] = bp[-(8 * (r >> 2) + (r & 3))];
         }
-        auto product = [&](unsigned tile, const u32x4 (&f)[NK], f32x16& x) {  // x += rows of the tile . f
-          constexpr int GK = 4;
+        auto product = [&](unsigned tile, const auto& f, f32x16& x) {  // x += rows of the tile . f
+          constexpr int GK = WIDE ? 2 : 4;
           u32x4 af[GK];
 #pragma unroll
           for (int c = 0; c < NK; c += GK) {
 #pragma unroll
-            for (int ks = 0; ks < GK && c + ks < NK; ++ks) af[ks] = at.frag(tile, 32 * u, c + ks);
+            for (int ks = 0; ks < GK && c + ks < NK; ++ks) af[ks] = in.frag(tile, 32 * u, c + ks);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int ks = 0; ks < GK && c + ks < NK; ++ks) x = E::mma(af[ks], f[c + ks], x);
@@ -1113,7 +1131,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
           for (int kk = 0; kk < 2; ++kk) {
             u32x4 af[ND];
 #pragma unroll
-            for (int d = 0; d < ND; ++d) af[d] = at.frag_t(tile, 32 * u + 16 * kk, d);
+            for (int d = 0; d < ND; ++d) af[d] = in.frag_t(tile, 32 * u + 16 * kk, d);
             const u32x4 xb = pack8<E>(x, 8 * kk);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -1122,15 +1140,32 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
         };
         product(qt, kf, s);
         f32x4 ls[4];
+        auto logs = [&] {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) ls[q] = *reinterpret_cast<const f32x4*>(lt + 32 * u + 8 * q + 4 * hi);
+          for (int q = 0; q < 4; ++q) ls[q] = *reinterpret_cast<const f32x4*>(lt + 32 * u + 8 * q + 4 * hi);
+        };
+        if (!WIDE) logs();
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const f32x4 y = *reinterpret_cast<const f32x4*>(lt + 64 + 32 * u + 8 * q + 4 * hi);
 #pragma unroll
           for (int r = 0; r < 4; ++r) dp[4 * q + r] = y[r];
         }
-        product(ot, vf, dp);
+        if constexpr (WIDE) {
+          constexpr int GK = 2;
+          u32x4 af[GK], bf[GK];
+#pragma unroll
+          for (int c = 0; c < NK; c += GK) {
+#pragma unroll
+            for (int ks = 0; ks < GK; ++ks) af[ks] = in.frag(ot, 32 * u, c + ks), bf[ks] = in.frag(lV, 0, c + ks);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks < GK; ++ks) dp = E::mma(af[ks], bf[ks], dp);
+          }
+        } else {
+          product(ot, vf, dp);
+        }
+        if (WIDE) logs();
         if (a.causal && j0 + 31 > p0) {
           const int lim = j - p0 - 4 * hi;  // queries before it do not see the key
 #pragma unroll
@@ -1177,7 +1212,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
       }
     return;
   }
-  const bool in = j < sq.klen;  // rows behind the sequence get zeros
+  const bool key = j < sq.klen;  // rows behind the sequence get zeros
   uint16_t* const kp = a.dk + b * a.sdk.b + (int64_t)j * a.sdk.t + hk * a.sdk.h;
   uint16_t* const vp = a.dv + b * a.sdv.b + (int64_t)j * a.sdv.t + hk * a.sdv.h;
 #pragma unroll
@@ -1188,7 +1223,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void rb_dkv_kernel(RbArgs a
       if (c >= a.D) continue;
       float x[8];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = in ? dk[d][4 * g + r] * a.scale : 0.f, x[4 + r] = in ? dv[d][4 * g + r] : 0.f;
+      for (int r = 0; r < 4; ++r) x[r] = key ? dk[d][4 * g + r] * a.scale : 0.f, x[4 + r] = key ? dv[d][4 * g + r] : 0.f;
       store4<E>(kp + c, x[0], x[1], x[2], x[3]);
       store4<E>(vp + c, x[4], x[5], x[6], x[7]);
     }
