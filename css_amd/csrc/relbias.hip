@@ -21,6 +21,7 @@ typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 
 constexpr float RB_LOG2E = 1.4426950408889634f, RB_LN2 = 0.6931471805599453f;
 constexpr int RB_PAD = 96;          // entries of the spread table beyond the largest distance on each side: a 64 x 32 tile that
@@ -248,10 +249,10 @@ template <int DP>
 struct LaneAt {
   static constexpr unsigned P = 2 * DP;
   unsigned row, tr;
-  __device__ __forceinline__ explicit LaneAt(int lane) {
+  __device__ __forceinline__ LaneAt(const void* smem, int lane) {  // tiles are then named by their offset in smem (at LDS address 0)
     const int l16 = lane & 15, hi = lane >> 5;
-    row = tile_at<DP>(lane & 31, hi);
-    tr = tile_at<DP>(4 * hi + (l16 >> 2), ((lane >> 4) & 1) * 2 + ((l16 & 3) >> 1)) + (l16 & 1) * 8;
+    row = lds_addr(smem) + tile_at<DP>(lane & 31, hi);
+    tr = lds_addr(smem) + tile_at<DP>(4 * hi + (l16 >> 2), ((lane >> 4) & 1) * 2 + ((l16 & 3) >> 1)) + (l16 & 1) * 8;
   }
   // Makes the compiler derive the other addresses here: held over the loop they do not fit the registers beside 128 columns, and
   // a reload from scratch waits for the tiles under way as well.
@@ -327,7 +328,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
   dk.init(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, 0, sq.klen, a.D, wave, lane);
   dv.init(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, 0, sq.klen, a.D, wave, lane);
   const unsigned lK = lds_addr(sK), lV = lds_addr(sV);
-  const LaneAt<DP> in(lane);
+  const LaneAt<DP> in(smem, lane);
   if (nt > 0) {
     dk.next(lK, wave);
     dv.next(lV, wave);
@@ -354,7 +355,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
       dv.next(lV + (buf ^ 1) * TILE, wave);
     };
     if (j0 < wend) {
-      const unsigned kt = lK + buf * TILE, vt = lV + buf * TILE;
+      constexpr unsigned kt = buf * TILE, vt = (2 + buf) * TILE;
       f32x16 s[2];
       // S^T = K Q^T + bias.  Operands are requested in groups ahead of the products that use them: left alone, the compiler
       // reads, waits and multiplies one fragment at a time.
@@ -477,8 +478,7 @@ __global__ __launch_bounds__(64 * NW, 2) void rb_few_kernel(RbArgs a) {
   constexpr int P = 2 * DP, NK = DP / 16, ND = DP / 32, CPR = DP / 8, RPI = 64 / CPR, NV = 32 / RPI, NT = 64 * NW;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   unsigned char* const sV = smem + wave * 32 * P;
-  const unsigned lV = lds_addr(sV);
-  const LaneAt<DP> at(lane);
+  const LaneAt<DP> at(smem, lane);
   float* const sT = reinterpret_cast<float*>(smem + few_area<DP, NW>());
   const int G = a.per_group.d, R = a.Tq * G;
   const int id = xcd_order(blockIdx.x, a.nblk);
@@ -598,7 +598,7 @@ __global__ __launch_bounds__(64 * NW, 2) void rb_few_kernel(RbArgs a) {
       const u32x4 rest = pack8<E>(s, 8 * kk);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        const u32x4 vf = at.frag_t(lV, 16 * kk, d);
+        const u32x4 vf = at.frag_t(wave * 32 * P, 16 * kk, d);
         o[d] = E::mma(vf, pb, o[d]);
         o[d] = E::mma(vf, rest, o[d]);
       }
@@ -753,7 +753,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
   dK.init(a.k + b * a.sk.b + hk * a.sk.h, a.sk.t, ta, sq.klen, a.D, wave, lane);
   dV.init(a.v + b * a.sv.b + hk * a.sv.h, a.sv.t, ta, sq.klen, a.D, wave, lane);
   const unsigned lK = lds_addr(sK), lV = lds_addr(sV);
-  LaneAt<DP> in(lane);
+  LaneAt<DP> in(smem, lane);
   if (ta < nt) {
     dK.next(lK, wave);
     dV.next(lV, wave);
@@ -817,7 +817,7 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
       dV.next(lV + (buf ^ 1) * TILE, wave);
     };
     if (!(j0 < wend)) transfer();
-    const unsigned kt = lK + buf * TILE, vt = lV + buf * TILE;
+    constexpr unsigned kt = buf * TILE, vt = (2 + buf) * TILE;
     const bool active = j0 < wend;
     const bool near = active && j0 - (p0 + 31) < a.mde && j0 + 63 - p0 > -a.mde;
     const int pw = sq.off + q0;
@@ -1044,8 +1044,9 @@ __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
   const int per = k0 < sq.klen ? max((sq.qlen + ROWS - 1) / ROWS - t0, 0) : 0, steps = per * G;
   const int it0 = (int)((int64_t)steps * part / a.nsplit), it1 = (int)((int64_t)steps * (part + 1) / a.nsplit);
   const unsigned lQ = lds_addr(sQ), lO = lds_addr(sO);
-  LaneAt<DP> in(lane);
-  const unsigned lV = lds_addr(sV) + wave * 32 * P;
+  LaneAt<DP> in(smem, lane);
+  const unsigned stats = lds_addr(sL) + hi * 16;   // row statistics: a lane reads four rows at a time
+  const unsigned mine = 4 * TILE + wave * 32 * P;  // the wave's keys of V
   if constexpr (WIDE) {
     if (it0 < it1) {  // arrives with the first tile
       TileDma<DP> dV;
@@ -1088,8 +1089,7 @@ __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
       constexpr int buf = decltype(parity)::value;
       const bool more = t + 1 < tb;
       if (more) load(t + 1, buf ^ 1);
-      const unsigned qt = lQ + buf * TILE, ot = lO + buf * TILE;
-      const float* const lt = sL + buf * 128;
+      constexpr unsigned qt = buf * TILE, ot = (2 + buf) * TILE;
       if constexpr (E::narrow) {  // one factor for all of dK's sum so far: a tile of larger gradients takes it down
         const float top = sF[buf], f = row_factor(top);
         if (top > 0.f && f < fac) {
@@ -1106,7 +1106,19 @@ __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
         const int p0 = sq.off + t * ROWS + 32 * u;  // position of the sub-tile's first query
         if (j0 >= sq.klen || (a.causal && j0 > p0 + 31)) continue;
         if (WIDE) in.renew();
+        // The operands in the order of their products, requested RING ahead: rows of q, rows of dout (WIDE: each with its piece of
+        // V), dout transposed, q transposed.  The exponentials stand between the products of dP, P (dP - delta) between those of dV.
+        constexpr int ROW2 = WIDE ? 2 * NK : NK, N2 = NK + ROW2, N3 = N2 + 2 * ND, N4 = N3 + 2 * ND, RING = WIDE ? 4 : 6;
+        auto fetch = [&](int n) {
+          if (n < NK) return in.frag(qt, 32 * u, n);
+          if (n < N2) return WIDE && (n & 1) ? in.frag(mine, 0, (n - NK) >> 1) : in.frag(ot, 32 * u, WIDE ? (n - NK) >> 1 : n - NK);
+          const int x = n < N3 ? n - N2 : n - N3;
+          return in.frag_t(n < N3 ? ot : qt, 32 * u + 16 * (x / ND), x % ND);
+        };
+        auto row4 = [&](int first) { return *(const lds_f32x4*)(uintptr_t)(stats + (buf * 128 + 32 * u + first) * 4); };
+        u32x4 ring[RING];
         f32x16 s, dp;
+        f32x4 ls[4];
         if (j0 - (p0 + 31) >= a.mde || j0 + 31 - p0 <= -a.mde) {
           s = splat16(j0 > p0 ? right : left);
         } else {
@@ -1114,71 +1126,68 @@ __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] = bp[-(8 * (r >> 2) + (r & 3))];
         }
-        auto product = [&](unsigned tile, const auto& f, f32x16& x) {  // x += rows of the tile . f
-          constexpr int GK = WIDE ? 2 : 4;
-          u32x4 af[GK];
 #pragma unroll
-          for (int c = 0; c < NK; c += GK) {
+        for (int n = 0; n < RING; ++n) ring[n] = fetch(n);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int ks = 0; ks < GK && c + ks < NK; ++ks) af[ks] = in.frag(tile, 32 * u, c + ks);
-            __builtin_amdgcn_sched_barrier(0);
+        for (int n = 0; n < NK; ++n) {
+          s = E::mma(ring[n % RING], kf[n], s);
+          ring[n % RING] = fetch(n + RING);
+          if (n % (NK / 2) == 0) {
 #pragma unroll
-            for (int ks = 0; ks < GK && c + ks < NK; ++ks) x = E::mma(af[ks], f[c + ks], x);
+            for (int g = 4 * n / NK; g < 4 * n / NK + 2; ++g) {
+              const f32x4 y = row4(64 + 8 * g);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) dp[4 * g + r] = y[r];
+            }
           }
-        };
-        auto outer = [&](unsigned tile, const f32x16& x, f32x16 (&sum)[ND]) {  // sum += tile^T . x, x rounded here
-#pragma unroll
-          for (int kk = 0; kk < 2; ++kk) {
-            u32x4 af[ND];
-#pragma unroll
-            for (int d = 0; d < ND; ++d) af[d] = in.frag_t(tile, 32 * u + 16 * kk, d);
-            const u32x4 xb = pack8<E>(x, 8 * kk);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int d = 0; d < ND; ++d) sum[d] = E::mma(af[d], xb, sum[d]);
-          }
-        };
-        product(qt, kf, s);
-        f32x4 ls[4];
-        auto logs = [&] {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) ls[q] = *reinterpret_cast<const f32x4*>(lt + 32 * u + 8 * q + 4 * hi);
-        };
-        if (!WIDE) logs();
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 y = *reinterpret_cast<const f32x4*>(lt + 64 + 32 * u + 8 * q + 4 * hi);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) dp[4 * q + r] = y[r];
+          __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (WIDE) {
-          constexpr int GK = 2;
-          u32x4 af[GK], bf[GK];
-#pragma unroll
-          for (int c = 0; c < NK; c += GK) {
-#pragma unroll
-            for (int ks = 0; ks < GK; ++ks) af[ks] = in.frag(ot, 32 * u, c + ks), bf[ks] = in.frag(lV, 0, c + ks);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int ks = 0; ks < GK; ++ks) dp = E::mma(af[ks], bf[ks], dp);
-          }
-        } else {
-          product(ot, vf, dp);
-        }
-        if (WIDE) logs();
         if (a.causal && j0 + 31 > p0) {
           const int lim = j - p0 - 4 * hi;  // queries before it do not see the key
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (8 * (r >> 2) + (r & 3) < lim) s[r] = -RB_INF;
         }
+        constexpr int EACH = 16 / NK;  // exponentials behind a product; their rows' sums are requested two products ahead
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, -ls[r >> 2][r & 3]));
-          dp[r] *= E::narrow ? s[r] * fac : s[r];
+        for (int g = 0; g < 4; ++g)
+          if (4 * g < 2 * EACH) ls[g] = row4(8 * g);
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+          if constexpr (WIDE) {
+            const int x = NK + 2 * n;
+            dp = E::mma(ring[x % RING], ring[(x + 1) % RING], dp);
+            ring[x % RING] = fetch(x + RING);
+            ring[(x + 1) % RING] = fetch(x + 1 + RING);
+          } else {
+            dp = E::mma(ring[(NK + n) % RING], vf[n], dp);
+            ring[(NK + n) % RING] = fetch(NK + n + RING);
+          }
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            if (4 * g >= (n + 2) * EACH && 4 * g < (n + 3) * EACH) ls[g] = row4(8 * g);
+#pragma unroll
+          for (int r = n * EACH; r < (n + 1) * EACH; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, -ls[r >> 2][r & 3]));
+          __builtin_amdgcn_sched_barrier(0);
         }
-        outer(ot, s, dv);
-        outer(qt, dp, dk);
+        u32x4 xb[2] = {pack8<E>(s, 0), pack8<E>(s, 8)};
+#pragma unroll
+        for (int n = 0; n < 2 * ND; ++n) {
+          dv[n % ND] = E::mma(ring[(N2 + n) % RING], xb[n / ND], dv[n % ND]);
+          if (N2 + n + RING < N4) ring[(N2 + n) % RING] = fetch(N2 + n + RING);
+          constexpr int M = 8 / ND;
+#pragma unroll
+          for (int r = n * M; r < (n + 1) * M; ++r) dp[r] *= E::narrow ? s[r] * fac : s[r];
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        xb[0] = pack8<E>(dp, 0), xb[1] = pack8<E>(dp, 8);
+#pragma unroll
+        for (int n = 0; n < 2 * ND; ++n) {
+          dk[n % ND] = E::mma(ring[(N3 + n) % RING], xb[n / ND], dk[n % ND]);
+          if (N3 + n + RING < N4) ring[(N3 + n) % RING] = fetch(N3 + n + RING);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
       if (more) store(buf ^ 1);
       dma_wait();
