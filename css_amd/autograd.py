@@ -196,13 +196,14 @@ class MhaRelBias(torch.autograd.Function):
         q, k, v, table, out, lse, offsets, k_lens, q_lens = ctx.saved_tensors
         buckets, scale, causal, offset = ctx.how
         grads = ob.mha_relbias_bwd(q, k, v, table, out, lse, dout, buckets, scale=scale, causal=causal,
-                                        offset=offset if offsets is None else offsets, k_lens=k_lens, q_lens=q_lens)
+                                   offset=offset if offsets is None else offsets, k_lens=k_lens, q_lens=q_lens)
         return (*grads, None, None, None, None, None, None)
 
 
 def mha_relbias(q, k, v, table, buckets, *, scale=None, causal=False, offset=0, k_lens=None, q_lens=None):
     """ops.mha_relbias under autograd: out, differentiable in q, k, v and the bias table (arguments as there).  Rows behind a
-    sequence's end get zero gradients, whatever arrives from above for them."""
+    sequence's end get zero gradients, whatever arrives from above for them.  In a captured graph: forward and backward of one
+    capture, on leaves that no eager autograd graph still holds (else torch ties the capture to the eager stream and fails it)."""
     return MhaRelBias.apply(q, k, v, table, buckets, scale, causal, offset, k_lens, q_lens)
 
 

@@ -303,7 +303,14 @@ DEV void store_rows(const RbArgs& a, const f32x16 (&o)[DP / 32], float m, float 
 }
 
 // =============================================================================================== forward
-// One workgroup = 4 waves x 32 queries of one (sequence, head); 64-key tiles of K and V, double buffered in LDS.
+// One workgroup = 4 waves x 32 queries of one (sequence, head); 64-key tiles of K and V, double buffered in LDS, softmax in one pass
+// with a running maximum and sum in f32.  P is rounded to the tensors' type as the second product's operand (half a step of each
+// term, while the sum that divides it is not rounded): f32 operands would take eight times the matrix unit's time.
+// Bound by the vector unit at 64 columns: a score takes an exponential (8 cycles a wave) and some four instructions beside its
+// 128 flops, and the two units run side by side only across waves.  11250 x 11250, 8 heads of 64: 322 us, 805 TFLOP/s (a large
+// matrix product reaches 1178 here); 2 x 2047 causal, 16 heads of 128: 55 us, 625 TFLOP/s; 32 x 400, 4 heads: 15.4 us, of which some
+// 3.4 pass before the first product.  Scores of the next tile issued ahead of this one's exponentials took 496 us for the long
+// case: the registers of both tiles do not fit beside two waves.
 template <class E, int DP>
 __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -465,8 +472,10 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
 // Rows = (query, head of the group) of one (sequence, key head), 32 to a workgroup: a head's group shares the K and V it reads.
 // Nothing is reused across waves, so each of the NW waves streams its own 32-key tiles (every NW-th of the workgroup's), K straight
 // into operand registers, V through a wave's own LDS tile for the transposing reads, the next tile's loads in flight; the waves'
-// running softmax states are joined in LDS.  Bound by the bytes of K and V.  Where few workgroups would run, the keys are split
-// over `nsplit` of them: states go to the workspace and rb_join_kernel joins them in order.
+// running softmax states are joined in LDS.  Bound by the bytes of K and V: 32 x 1 against up to 8192 keys, 16 heads in groups of 4,
+// 128 columns: 95.7 us, 4.16 TB/s (a large copy reaches 5.16); 4 x 8 x 30001, 8 heads of 64: 53.5 us, 4.6 TB/s; 1 x 500, 4 heads:
+// 11.7 us, one workgroup's chain of loads.  Where few workgroups would run, the keys are split over `nsplit` of them: states go
+// to the workspace and rb_join_kernel joins them in order (4.8 us for the first of these).
 constexpr int RB_FEW_TABLE = 4096;  // floats of LDS for the group's tables by distance; wider ones are gathered from memory
 template <int DP, int NW>
 constexpr int few_area() {  // bytes: the waves' V tiles, later their O rows [NW][32][DP + 4] and (reference, sum) [NW][2][32]
@@ -722,6 +731,12 @@ DEV float swap_halves(float x) {
 
 // dq and the table's gradient: 4 waves x 32 queries of one (sequence, head) against 64-key tiles.
 //   S^T = K Q^T (+ bias), dP^T = V dO^T (from -delta), dS = P dP, dQ^T += K^T dS^T
+// dS is rounded to the tensors' type for the last product only; the table's gradient takes it in f32.  dk and dv have a kernel of
+// their own, which computes S and dP again (7 products for 5): sums over queries and over keys in one kernel would need atomics,
+// and results that change from run to run, or a T x T operand in memory.
+// Bound by stalls between the products: the vector unit is busy for 42% of the 6001 x 6001 case, the matrix unit for 29%, not at
+// the same time, with 1.5 waves a SIMD.  That case (8 heads of 64) 163 us, 680 TFLOP/s of its three products; 2 x 2047 causal,
+// 16 heads of 128: 85 us (125 with the operands' addresses held in registers, which did not fit); 32 x 400, 4 heads: 27 us.
 // Where few workgroups would run, the keys are split over `nsplit` of them, whose sums rb_dq_join_kernel adds in order.
 // It also leaves delta_i = do_i . o_i and the rows' log-sum-exp in log2 units for the next kernel, +inf where a row has no
 // keys or lies behind its sequence (exp2(s - inf) = 0: such rows drop out of every product).
@@ -1009,8 +1024,11 @@ DEV void table_sum(const RbArgs& a, int entry, int nwg) {
 
 // dk and dv: 4 waves x 32 keys of one (sequence, key head) against 64-query tiles of every head of its group.
 //   S = Q K^T (+ bias), dV^T += dO^T P, dP = dO V^T (from -delta), dK^T += Q^T dS
-// (at a head width of 128 K, V and the sums are 192 registers: one wave a SIMD with 512; two waves spill, 357 us against 95 for the
-// causal 2 x 2047 case).  Where few workgroups would run, the (head, query tile) steps are split over `nsplit`
+// P and dS are rounded to the tensors' type as operands, the sums are f32.  Operands are requested ahead of their products through
+// a whole sub-tile, which else waited for LDS twelve times (6001 x 6001, 8 heads of 64: 214 -> 203 us, 725 TFLOP/s of its four products).
+// WIDE: K and the sums are 160 of 256 registers, V stays in LDS and tiles have 32 rows (2 x 2047 causal, 4 key heads of 128: 91 us,
+// 750 TFLOP/s; with V in registers one wave a SIMD remains: 107).  32 x 400, 4 heads: 27 us.  Bound, as the dq kernel, by what
+// two waves a SIMD cannot hide.  Where few workgroups would run, the (head, query tile) steps are split over `nsplit`
 // workgroups, whose sums rb_dkv_join_kernel adds in order.
 template <class E, int DP>
 __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
@@ -1372,7 +1390,8 @@ int launch_fwd(RbArgs a, const csship_relbias* p, hipStream_t s) {
 }
 
 // Workgroups of the dk / dv kernel take 128 keys of a sequence and key head; where those leave most of the chip idle, each one's
-// steps (64 queries of one head) are split, at most 8 ways and not below 8 steps.
+// steps (64 queries of one head) are split, up to 512 workgroups and not below 4 steps (2 x 2047 causal, 4 key heads of 128,
+// backward: 189 us; up to 256: 227, up to 768: 190; 1 x 3000, 8 heads sharing one key head: 122, 128, 129).
 int dkv_splits(const csship_relbias* p) {
   const int64_t wgs = (int64_t)p->B * p->Hk * ((p->Tk + 127) / 128), steps = (int64_t)(p->H / p->Hk) * ((p->Tq + 63) / 64);
   if (wgs == 0) return 1;
@@ -1380,7 +1399,8 @@ int dkv_splits(const csship_relbias* p) {
   return (int)(want < 1 || most < 1 ? 1 : want < most ? want : most);
 }
 
-// The same for the dq kernel's 128 queries and their keys (64 at a time), not below 4 steps.
+// The same for the dq kernel's 128 queries and their keys (64 at a time), up to 768 workgroups and not below 2 steps
+// (6001 x 6001, 8 heads, backward: 333 us; up to 512, no split there: 341).
 int dq_splits(const csship_relbias* p) {
   const int64_t wgs = (int64_t)p->B * p->H * ((p->Tq + 127) / 128), steps = (p->Tk + 63) / 64;
   if (wgs == 0) return 1;

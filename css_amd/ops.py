@@ -371,7 +371,7 @@ def _relbias_pack(q, k, v, table, buckets, scale, causal, offset, k_lens, q_lens
     each = 0
     if isinstance(offset, torch.Tensor):
         offset, each = 0, _relbias_words(offset, "offset", B, q)
-    elif not -(1 << 28) <= offset <= 1 << 28:
+    elif offset != int(offset) or not -(1 << 28) <= offset <= 1 << 28:
         raise RuntimeError(f"css_amd: offset {offset} out of range")
     scale = D ** -0.5 if scale is None else float(scale)
     if not 1e-6 < scale < 1e6:

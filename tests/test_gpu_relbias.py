@@ -187,6 +187,23 @@ def test_padded_batch_reads_nothing_behind_its_ends(lib, dtype, causal):
             assert (got[name][b, n:] == 0).all(), name
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [False, True])
+def test_padded_batch_of_wide_heads(lib, dtype, causal):
+    """the same at 120 columns, where tiles of the key gradients have 32 rows; groups of three heads, steps split over workgroups"""
+    lens = [190, 0, 1, 31, 32, 33, 96, 161]
+    q, k, v, table, do = make(13, dtype, len(lens), 190, 190, 6, 2, 120, 32)
+    for b, n in enumerate(lens):
+        for i, x in enumerate((q, k, v, do)):
+            x[b, n:] = (math.inf, math.nan, math.nan, -math.inf)[i]
+    kl = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    out, lse, got = check_all(lib, q, k, v, table, do, (32, 128), causal=causal, k_lens=kl, q_lens=kl)
+    for b, n in enumerate(lens):
+        assert (out[b, n:] == 0).all() and (lse[b, :, n:] == -math.inf).all()
+        for name in ("dq", "dk", "dv"):
+            assert (got[name][b, n:] == 0).all(), name
+
+
 def test_serving_batch_of_single_frames(lib):
     """few rows, split keys, lengths and offsets per sequence; an idle slot and garbage behind the kept keys"""
     lens = [1700, 1, 0, 1024, 33, 1699]
@@ -445,6 +462,7 @@ def test_refusals(lib):
         (TypeError, (q, k, v, table, ok), dict(q_lens=[1, 2])),
         (RuntimeError, (q, k, v, table, ok), dict(offset=lens.cpu())),
         (RuntimeError, (q, k, v, table, ok), dict(offset=1 << 30)),
+        (RuntimeError, (q, k, v, table, ok), dict(offset=0.5)),
         (RuntimeError, (q, k, v, table, ok), dict(scale=0.0)),
     ]
     for kind, args, how in bad:
