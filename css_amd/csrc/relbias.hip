@@ -307,7 +307,7 @@ DEV void store_rows(const RbArgs& a, const f32x16 (&o)[DP / 32], float m, float 
 // with a running maximum and sum in f32.  P is rounded to the tensors' type as the second product's operand (half a step of each
 // term, while the sum that divides it is not rounded): f32 operands would take eight times the matrix unit's time.
 // Bound by the vector unit at 64 columns: a score takes an exponential (8 cycles a wave) and some four instructions beside its
-// 128 flops, and the two units run side by side only across waves.  11250 x 11250, 8 heads of 64: 322 us, 805 TFLOP/s (a large
+// 128 flops, and the two units run side by side only across waves.  11250 x 11250, 8 heads of 64: 317 us, 818 TFLOP/s (a large
 // matrix product reaches 1178 here); 2 x 2047 causal, 16 heads of 128: 55 us, 625 TFLOP/s; 32 x 400, 4 heads: 15.4 us, of which some
 // 3.4 pass before the first product.  Scores of the next tile issued ahead of this one's exponentials took 496 us for the long
 // case: the registers of both tiles do not fit beside two waves.
