@@ -734,14 +734,18 @@ DEV float swap_halves(float x) {
 // dS is rounded to the tensors' type for the last product only; the table's gradient takes it in f32.  dk and dv have a kernel of
 // their own, which computes S and dP again (7 products for 5): sums over queries and over keys in one kernel would need atomics,
 // and results that change from run to run, or a T x T operand in memory.
-// Bound by stalls between the products: the vector unit is busy for 42% of the 6001 x 6001 case, the matrix unit for 29%, not at
-// the same time, with 1.5 waves a SIMD.  That case (8 heads of 64) 163 us, 680 TFLOP/s of its three products; 2 x 2047 causal,
-// 16 heads of 128: 85 us (125 with the operands' addresses held in registers, which did not fit); 32 x 400, 4 heads: 27 us.
+// Bound by both units in turn: 6001 x 6001, 8 heads of 64: 141 us, 785 TFLOP/s of its three products, the vector unit busy for 59%
+// of the time, the matrix unit for 42%.  2 x 2047 causal, 16 heads of 128: 85 us (125 with the operands' addresses held in
+// registers, which did not fit); 32 x 400, 4 heads: 27 us.
 // Where few workgroups would run, the keys are split over `nsplit` of them, whose sums rb_dq_join_kernel adds in order.
 // It also leaves delta_i = do_i . o_i and the rows' log-sum-exp in log2 units for the next kernel, +inf where a row has no
 // keys or lies behind its sequence (exp2(s - inf) = 0: such rows drop out of every product).
-template <class E, int DP>
-__global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
+// WAVES a SIMD: 64 columns fit three (fewer operands ahead, addresses derived per sub-tile), for more than two workgroups a CU
+// (6001 x 6001, whole backward: 326 us against 340); up to there the wider form is faster (24 ragged windows: 36.4 us
+// against 37.6; 32 x 400: 54.1 against 54.9, eager calls).
+template <class E, int DP, int WAVES>
+__global__ __launch_bounds__(256, WAVES) void rb_dq_kernel(RbArgs a) {
+  constexpr bool TIGHT = DP == 128 || WAVES == 3;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   constexpr int P = 2 * DP, TILE = 64 * P, NK = DP / 16, ND = DP / 32;
   unsigned char* const sK = smem;
@@ -852,11 +856,11 @@ __global__ __launch_bounds__(256, 2) void rb_dq_kernel(RbArgs a) {
     for (int u = 0; u < 2; ++u) {
       if (u == 1 && any_near) __syncthreads();
       if (!active) continue;
-      if (DP == 128) in.renew();
+      if (TIGHT) in.renew();
       f32x16 s, dp = splat16(-delta);
       // operands in groups ahead of the products that use them, as in rb_fwd_kernel
       auto scores = [&](auto zero) {
-        constexpr int GK = DP == 128 ? 2 : 4;
+        constexpr int GK = TIGHT ? 2 : 4;
         u32x4 kf[GK], vf[GK];
 #pragma unroll
         for (int c = 0; c < NK; c += GK) {
@@ -1027,8 +1031,8 @@ DEV void table_sum(const RbArgs& a, int entry, int nwg) {
 // P and dS are rounded to the tensors' type as operands, the sums are f32.  Operands are requested ahead of their products through
 // a whole sub-tile, which else waited for LDS twelve times (6001 x 6001, 8 heads of 64: 214 -> 203 us, 725 TFLOP/s of its four products).
 // WIDE: K and the sums are 160 of 256 registers, V stays in LDS and tiles have 32 rows (2 x 2047 causal, 4 key heads of 128: 91 us,
-// 750 TFLOP/s; with V in registers one wave a SIMD remains: 107).  32 x 400, 4 heads: 27 us.  Bound, as the dq kernel, by what
-// two waves a SIMD cannot hide.  Where few workgroups would run, the (head, query tile) steps are split over `nsplit`
+// 750 TFLOP/s; with V in registers one wave a SIMD remains: 107).  32 x 400, 4 heads: 27 us.  Both units are busy for 35% of the
+// 6001 x 6001 case: its 376 workgroups leave every second SIMD with one wave, and 220 registers allow no third.  Where few workgroups would run, the (head, query tile) steps are split over `nsplit`
 // workgroups, whose sums rb_dkv_join_kernel adds in order.
 template <class E, int DP>
 __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
@@ -1400,7 +1404,7 @@ int dkv_splits(const csship_relbias* p) {
 }
 
 // The same for the dq kernel's 128 queries and their keys (64 at a time), up to 768 workgroups and not below 2 steps
-// (6001 x 6001, 8 heads, backward: 333 us; up to 512, no split there: 341).
+// (6001 x 6001, 8 heads, backward: 333 us; up to 512, no split there: 341; both with two waves a SIMD).
 int dq_splits(const csship_relbias* p) {
   const int64_t wgs = (int64_t)p->B * p->H * ((p->Tq + 127) / 128), steps = (p->Tk + 63) / 64;
   if (wgs == 0) return 1;
@@ -1416,7 +1420,9 @@ int launch_bwd(RbArgs a, const csship_relbias* p, hipStream_t s) {
   a.nqtile = a.ntile * a.nsplit;
   a.nblk = a.B * a.H * a.nqtile;
   if (a.nblk > 0) {
-    if (const int rc = launch(rb_dq_kernel<E, DP>, a.nblk, dq_lds(DP, a.mde), a, a.H, s)) return rc;
+    const int rc = DP == 64 && a.nblk > 512 ? launch(rb_dq_kernel<E, DP, DP == 64 ? 3 : 2>, a.nblk, dq_lds(DP, a.mde), a, a.H, s)
+                                            : launch(rb_dq_kernel<E, DP, 2>, a.nblk, dq_lds(DP, a.mde), a, a.H, s);
+    if (rc) return rc;
     if (a.nsplit > 1)
       if (const int rc = launch(rb_dq_join_kernel<E, DP>, ((int64_t)a.B * a.H * a.Tq * (DP / 4) + 255) / 256, 0, a, a.H, s)) return rc;
   }

@@ -274,11 +274,11 @@ def test_same_bits_every_time(lib):
         assert all(torch.equal(a, b) for a, b in zip(first, got))
 
 
-@pytest.mark.parametrize("B,H,Hk,Tq,Tk,causal", [(8, 10, 5, 520, 520, True), (7, 11, 11, 300, 390, True), (9, 12, 4, 270, 270, False),
-                                                (1, 3, 3, 1400, 1400, True)])
-def test_many_workgroups(lib, B, H, Hk, Tq, Tk, causal):
+@pytest.mark.parametrize("B,H,Hk,Tq,Tk,D,causal", [(8, 10, 5, 520, 520, 32, True), (7, 11, 11, 300, 390, 32, True), (9, 12, 4, 270, 270, 32, False),
+                                                  (1, 3, 3, 1400, 1400, 32, True), (9, 12, 6, 520, 300, 64, False), (22, 6, 2, 520, 430, 56, True)])
+def test_many_workgroups(lib, B, H, Hk, Tq, Tk, D, causal):
     """hundreds of workgroups whose heads do not fall on the 256 or 32 of one round of the chip: every tile is taken, and once"""
-    q, k, v, table, do = make(12, torch.bfloat16, B, Tq, Tk, H, Hk, 32, 32)
+    q, k, v, table, do = make(12, torch.bfloat16, B, Tq, Tk, H, Hk, D, 32)
     stale = [torch.full((n,), float("nan"), device="cuda") for n in [1 << 24] * 4 + [1 << 17] * 16]     # what a tile left out shows
     del stale
     check_all(lib, q, k, v, table, do, (32, 128), causal=causal, offset=Tk - Tq)
