@@ -27,6 +27,7 @@ constexpr float RB_LOG2E = 1.4426950408889634f, RB_LN2 = 0.6931471805599453f;
 constexpr int RB_PAD = 96;          // entries of the spread table beyond the largest distance on each side: a 64 x 32 tile that
                                     // is not wholly beyond it reaches at most 64 + 32 - 2 further
 constexpr float RB_BIG = 1048576.f; // table entries at or below -2^20 ban their distances; entries above 2^20 count as 2^20
+constexpr int SPAN_MAX = 2 * (CSSHIP_RELBIAS_MAX_DISTANCE + RB_PAD) + 1;
 constexpr int RB_MAX_POS = 1 << 28;  // lengths and offsets stay below it: distances in 32 bits
 constexpr float RB_INF = __builtin_inff();
 
@@ -718,7 +719,9 @@ __global__ __launch_bounds__(256) void rb_join_kernel(RbArgs a) {
 // 32 keys before: lanes 0..2 of a half separate their own part (`own`, a chain that starts at their half) from what came
 // over, which is added to the part kept from 32 keys before, `kept`.  So each (group, half) writes 32 neighbouring cells of its own
 // array per sub-tile, cells that the other waves do not touch in the same step (their queries are 32 further): plain
-// read-add-write with a barrier per step, no atomics, and a fixed order.  11 vector instructions per group of four; ds_add_f32
+// read-add-write with a barrier per step, no atomics, and a fixed order.  The arrays are rings of 256 distances: a step's tile
+// touches 191, and the 64 that it leaves behind are added up and put away during the next one (arrays over all distances leave
+// one workgroup a CU for wide tables: 2 x 8 heads of 64, 1500 x 1500, 800 distances: backward 98 us against 119).  11 vector instructions per group of four; ds_add_f32
 // took 187 cycles per instruction here (124 us for the 32 x 400 backward's dq kernel).
 constexpr int DPP_WAVE_ROR1 = 0x13c, DPP_ROW_SHR1 = 0x111;
 DEV float from_below(float x) { return dpp_mov<DPP_WAVE_ROR1>(x); }      // lane l: the value of lane l - 1, lane 0: of lane 63
@@ -734,7 +737,7 @@ DEV float swap_halves(float x) {
 // dS is rounded to the tensors' type for the last product only; the table's gradient takes it in f32.  dk and dv have a kernel of
 // their own, which computes S and dP again (7 products for 5): sums over queries and over keys in one kernel would need atomics,
 // and results that change from run to run, or a T x T operand in memory.
-// Bound by both units in turn: 6001 x 6001, 8 heads of 64: 141 us, 785 TFLOP/s of its three products, the vector unit busy for 59%
+// Bound by both units in turn: 6001 x 6001, 8 heads of 64: 139 us, 800 TFLOP/s of its three products, the vector unit busy for 59%
 // of the time, the matrix unit for 42%.  2 x 2047 causal, 16 heads of 128: 85 us (125 with the operands' addresses held in
 // registers, which did not fit); 32 x 400, 4 heads: 27 us.
 // Where few workgroups would run, the keys are split over `nsplit` of them, whose sums rb_dq_join_kernel adds in order.
@@ -752,8 +755,9 @@ __global__ __launch_bounds__(256, WAVES) void rb_dq_kernel(RbArgs a) {
   unsigned char* const sV = smem + 2 * TILE;
   float* const sB = reinterpret_cast<float*>(smem + 4 * TILE);
   const int span = 2 * (a.mde + RB_PAD) + 1;
-  float* const sG = sB + span;                                      // [4 groups][2 halves][span]
-  double* const sFar = reinterpret_cast<double*>(smem + 4 * TILE + ((9 * span + 1) / 2 * 2) * 4);  // [4][2], [4]
+  float* const sSum = sB + span;                                    // [span] sums by distance
+  float* const sG = sSum + span;                                    // [4 groups][2 halves][256] the sums still open
+  double* const sFar = reinterpret_cast<double*>(smem + 4 * TILE + (span + 1) / 2 * 16 + 8192);  // [4][2], [4]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const Place at = place_of(a);
   const Quot bh = split(at.head, a.per_head);
@@ -786,7 +790,7 @@ __global__ __launch_bounds__(256, WAVES) void rb_dq_kernel(RbArgs a) {
     u32x4 of[NK];
     row_frags<DP>(a.o + b * a.so.b + h * a.so.h, a.so.t, q0 + wave * 32, sq.qlen, a.D, lane, of);
     const float given = a.lse_in[((int64_t)b * a.H + h) * a.Tq + min(i, a.Tq - 1)];
-    for (int x = tid; x < 8 * span; x += 256) sG[x] = 0.f;
+    for (int x = tid; x < span + 2048; x += 256) sSum[x] = 0.f;
     const float x = i < sq.qlen ? given : -RB_INF;
 #pragma unroll
     for (int ks = 0; ks < NK; ++ks)
@@ -824,8 +828,25 @@ __global__ __launch_bounds__(256, WAVES) void rb_dq_kernel(RbArgs a) {
   dma_wait();
   __syncthreads();
   const float left = sB[0], right = sB[span - 1];
-  // lane's cell for key base 0: its own class (half), or for lanes 0..2 the other half's, 32 keys before
-  const int cls = n32 < 3 ? hi ^ 1 : hi, cell0 = cls * span + 4 * cls + 3 - n32 - (n32 < 3 ? 32 : 0) - p0 + a.mde + RB_PAD;
+  // lane's distance for key base 0 and its class (half); lanes 0..2: of the other half, 32 keys before.  Open sums stand at
+  // (distance - base) mod 256 of their class and group: a step touches the 191 from `low` on.
+  const int cls = n32 < 3 ? hi ^ 1 : hi, dist0 = 4 * cls + 3 - n32 - (n32 < 3 ? 32 : 0) - p0;
+  float* const cells = sG + cls * 256;
+  const int pw = sq.off + q0;
+  auto cell = [&](int k, int g) { return cells + (2 * g * 256 + ((dist0 + k + 8 * g) & 255)); };
+  // the 64 distances that no later step touches, from all classes to sSum, by one wave
+  auto close = [&](int from) {
+    const int r = from + lane, x = r + a.mde + RB_PAD;
+    if (x < 0 || x >= span) return;
+    float y = 0.f;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      float* const at = sG + c * 256 + (r & 255);
+      y += *at;
+      *at = 0.f;
+    }
+    sSum[x] = y;
+  };
 
   auto step = [&](int t, auto parity) {
     constexpr int buf = decltype(parity)::value;
@@ -839,12 +860,13 @@ __global__ __launch_bounds__(256, WAVES) void rb_dq_kernel(RbArgs a) {
     constexpr unsigned kt = buf * TILE, vt = (2 + buf) * TILE;
     const bool active = j0 < wend;
     const bool near = active && j0 - (p0 + 31) < a.mde && j0 + 63 - p0 > -a.mde;
-    const int pw = sq.off + q0;
+    const int low = j0 - pw - 127;  // the step's smallest distance
+    if (t > ta && wave == (t & 3) && low - 64 <= a.mde + RB_PAD && low > -a.mde - RB_PAD) close(low - 64);
     const bool any_near = j0 - (pw + 127) < a.mde && j0 + 63 - pw > -a.mde;  // of any wave: they share the barrier
     if (!near && pending) {  // the last parts kept have nothing to wait for
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        if (n32 < 3) sG[2 * g * span + cell0 + j0 + 8 * g] += sign * kept[g];
+        if (n32 < 3) *cell(j0, g) += sign * kept[g];
 #pragma unroll
       for (int g = 0; g < 4; ++g) kept[g] = 0.f;
       pending = false;
@@ -902,14 +924,14 @@ __global__ __launch_bounds__(256, WAVES) void rb_dq_kernel(RbArgs a) {
       if (near) {
         float old[4];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) old[g] = sG[2 * g * span + cell0 + j0 + 32 * u + 8 * g];
+        for (int g = 0; g < 4; ++g) old[g] = *cell(j0 + 32 * u, g);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float all = s[4 * g + 3] + from_below(s[4 * g + 2] + from_below(s[4 * g + 1] + from_below(s[4 * g])));
           const float own = s[4 * g + 3] + from_below_row(s[4 * g + 2] + from_below_row(s[4 * g + 1]));
           const float x = n32 < 3 ? (all - own) + kept[g] : all;
           kept[g] = swap_halves(own);
-          sG[2 * g * span + cell0 + j0 + 32 * u + 8 * g] = __builtin_fmaf(sign, x, old[g]);
+          *cell(j0 + 32 * u, g) = __builtin_fmaf(sign, x, old[g]);
         }
         pending = true;
       } else {
@@ -945,7 +967,7 @@ __global__ __launch_bounds__(256, WAVES) void rb_dq_kernel(RbArgs a) {
   if (pending) {
 #pragma unroll
     for (int g = 0; g < 4; ++g)
-      if (n32 < 3) sG[2 * g * span + cell0 + nt * 64 + 8 * g] += sign * kept[g];
+      if (n32 < 3) *cell(nt * 64, g) += sign * kept[g];
   }
 
   if (i < a.Tq && a.nsplit > 1) {  // sums in f32: [split][sequence, head, query][DP]
@@ -977,15 +999,11 @@ __global__ __launch_bounds__(256, WAVES) void rb_dq_kernel(RbArgs a) {
   farr = sign * wave_total(farr);
   if (lane == 0) sFar[2 * wave] = farl, sFar[2 * wave + 1] = farr;
   __syncthreads();
+  if (ta < nt && wave < 3) close((nt - 1) * 64 - pw - 127 + 64 * wave);  // the last step's
+  __syncthreads();
   const int each = (span + 255) >> 8, first = tid * each;
   double mine = 0.;
-  for (int x = first; x < min(first + each, span); ++x) {
-    float y = 0.f;
-#pragma unroll
-    for (int c = 0; c < 8; ++c) y += sG[c * span + x];
-    sB[x] = y;
-    mine += (double)y;
-  }
+  for (int x = first; x < min(first + each, span); ++x) mine += (double)sSum[x];
   double upto = mine;  // inclusive over the wave, then over the workgroup
 #pragma unroll
   for (int w = 1; w < 64; w <<= 1) {
@@ -993,13 +1011,14 @@ __global__ __launch_bounds__(256, WAVES) void rb_dq_kernel(RbArgs a) {
     if (lane >= w) upto += y;
   }
   if (lane == 63) sFar[8 + wave] = upto;
-  __syncthreads();  // sG has been read: the running sums take its place
-  double* const run = reinterpret_cast<double*>(smem + 4 * TILE + (span + 1) / 2 * 8);  // [span + 1]
+  __syncthreads();
+  double* const run = reinterpret_cast<double*>(smem);  // [span + 1], where the tiles and, for narrow ones, sB were
+  static_assert(4 * TILE + 4 * SPAN_MAX >= 8 * (SPAN_MAX + 1), "run ends before sSum");
   upto -= mine;
   for (int w = 0; w < wave; ++w) upto += sFar[8 + w];
   for (int x = first; x < min(first + each, span); ++x) {
     run[x] = upto;
-    upto += (double)sB[x];
+    upto += (double)sSum[x];
     if (x == span - 1) run[span] = upto;
   }
   __syncthreads();
@@ -1337,7 +1356,7 @@ RbArgs to_args(const csship_relbias* p) {
 }
 
 size_t fwd_lds(int DP, int md) { return (size_t)4 * 64 * 2 * DP + (2 * (md + RB_PAD) + 1) * 4; }
-size_t dq_lds(int DP, int md) { return (size_t)4 * 64 * 2 * DP + (size_t)(9 * (2 * (md + RB_PAD) + 1) + 1) / 2 * 2 * 4 + 96; }
+size_t dq_lds(int DP, int md) { return (size_t)4 * 64 * 2 * DP + (size_t)(md + RB_PAD + 1) * 16 + 8192 + 96; }
 size_t dkv_lds(int DP, int md) { return fwd_lds(DP, md) + 1024 + 16; }
 
 // launches with more than 64 KB of LDS have to be allowed, per device: asked for at each such launch
