@@ -316,7 +316,8 @@ def relbias_buckets(buckets, device):
         for i, b in enumerate(m):
             r = i - key[2]
             rng[b] = [r if rng[b][0] == rng[b][1] else rng[b][0], r + 1]
-        got = _RELBIAS_BUCKETS[key] = (torch.tensor(m, dtype=torch.int16).to(device), torch.tensor(rng, dtype=torch.int32).to(device))
+        new = torch.tensor(m, dtype=torch.int16).to(device), torch.tensor(rng, dtype=torch.int32).to(device)
+        got = _RELBIAS_BUCKETS.setdefault(key, new)  # two threads may build: both take the pair that stays, launches hold its address
     return got
 
 
