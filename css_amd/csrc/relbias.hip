@@ -45,9 +45,8 @@ struct ElemBf {
   DEV float lo(unsigned u) { return __uint_as_float(u << 16); }
   DEV float hi(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
 };
-// fp16 reaches down to 2^-24 only.  P is at most 1 and what rounds to zero there is below 2^-25 of its row; dS has the size of
-// the incoming gradient, which may be far smaller than 1: it is multiplied by a power of two before it is rounded, and the
-// sums are divided by it (row_factor).
+// fp16 reaches from 2^-24 to 2^16 only.  P is at most 1 and what rounds to zero there is below 2^-25 of its row; dS has the size of
+// dout v / Tk, which may be anything: it is multiplied by a power of two before it is rounded, and the sums are divided by it (fit).
 struct ElemHf {
   static constexpr bool narrow = true;
   DEV f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
@@ -92,7 +91,7 @@ struct RbArgs {
   uint16_t *out, *dq, *dk, *dv;
   float *lse, *dtable;
   const float* lse_in;
-  float *delta, *lse2, *size, *part, *part2;  // workspace; delta (negated), lse2, size (sum of squares of dout's row) [B, H, tq128]
+  float *delta, *lse2, *part, *part2;  // workspace; delta (negated), lse2 [B, H, tq128]
   int B, Tq, Tk, H, Hk, D, nb, md, mde, causal, offset;  // mde: md, or the furthest distance that occurs
   float scale, inv_scale, c2;  // c2 = scale * log2(e)
   int ntile, nblk, nsplit, nqtile, tq128;     // row tiles per (sequence, head); workgroups; key ranges (rb_few_kernel)
@@ -180,10 +179,27 @@ DEV float half_sum(float x) {
   return __uint_as_float(a0) + __uint_as_float(a1);
 }
 
-// the power of two that brings a row of dout with this sum of squares to a norm of 1 .. 2 (1 for zeros and for what is not finite)
-DEV float row_factor(float squares) {
-  const int e = (int)((__float_as_uint(squares) >> 23) & 0xff) - 127;  // floor(log2)
-  return squares > 0.f && e < 128 ? __uint_as_float((unsigned)(127 - (max(min(e, 120), -120) >> 1)) << 23) : 1.f;
+// fp16: the values that a lane rounds for its column of a sum are multiplied by a power of two, `fac`, which starts as large as the
+// products allow (|dS| < 2^40: 2^120 in f32) and goes down, the sum with it, whenever a value x (multiplied already) reaches
+// 2^15: the largest is then in 2^9 .. 2^10.  So nothing overflows, and from 2^-23 of the column's largest value on, all keep
+// 11 bits; what is smaller is off by at most 2^-34 of that largest one.  Both half waves hold the same columns.
+constexpr float RB_FAC0 = 0x1p80f;
+template <int ND>
+DEV void fit(f32x16& x, f32x16 (&sum)[ND], float& fac) {
+  float top = fabsf(x[0]);
+#pragma unroll
+  for (int r = 1; r < 16; ++r) top = fmaxf(top, fabsf(x[r]));
+  top = half_max(top);
+  if (__any(top >= 32768.f)) {
+    const float down = top >= 32768.f ? __builtin_ldexpf(1.f, 9 + 127 - (int)(__float_as_uint(top) >> 23)) : 1.f;
+    fac *= down;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] *= down;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum[d][r] *= down;
+  }
 }
 DEV double wave_total(double x) {
 #pragma unroll
@@ -749,6 +765,7 @@ DEV float swap_halves(float x) {
 template <class E, int DP, int WAVES>
 __global__ __launch_bounds__(256, WAVES) void rb_dq_kernel(RbArgs a) {
   constexpr bool TIGHT = DP == 128 || WAVES == 3;
+  constexpr bool LATE = DP == 128 || (WAVES == 3 && E::narrow);  // no registers to hold K's columns across the exponentials
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   constexpr int P = 2 * DP, TILE = 64 * P, NK = DP / 16, ND = DP / 32;
   unsigned char* const sK = smem;
@@ -785,7 +802,7 @@ __global__ __launch_bounds__(256, WAVES) void rb_dq_kernel(RbArgs a) {
   row_frags<DP>(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, q0 + wave * 32, sq.qlen, a.D, lane, qf);
   row_frags<DP>(a.dout + b * a.sdo.b + h * a.sdo.h, a.sdo.t, q0 + wave * 32, sq.qlen, a.D, lane, df);
   const float sign = wave & 1 ? -1.f : 1.f;
-  float delta = 0.f, lse2 = RB_INF, fac = 1.f;  // fac: of the rounded dS (fp16)
+  float delta = 0.f, lse2 = RB_INF, fac = RB_FAC0;  // fac: of the rounded dS (fp16)
   {
     u32x4 of[NK];
     row_frags<DP>(a.o + b * a.so.b + h * a.so.h, a.so.t, q0 + wave * 32, sq.qlen, a.D, lane, of);
@@ -797,16 +814,6 @@ __global__ __launch_bounds__(256, WAVES) void rb_dq_kernel(RbArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) delta += E::lo(df[ks][e]) * E::lo(of[ks][e]) + E::hi(df[ks][e]) * E::hi(of[ks][e]);
     delta = half_sum(delta);
-    if constexpr (E::narrow) {
-      float squares = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < NK; ++ks)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) squares += E::lo(df[ks][e]) * E::lo(df[ks][e]) + E::hi(df[ks][e]) * E::hi(df[ks][e]);
-      squares = half_sum(squares);
-      fac = row_factor(squares);
-      if (hi == 0 && part == 0) a.size[((int64_t)b * a.H + h) * a.tq128 + i] = squares;
-    }
     if (x != -RB_INF) lse2 = x * RB_LOG2E;
     // The matrix unit's sums lean to the negative side by about 2^-25 each; over the 36 million pairs of a 6001 x 6001 head that
     // showed as 10^-5 of the table's gradient.  Odd waves therefore compute -dP (and all behind it), so that it cancels.
@@ -910,7 +917,7 @@ __global__ __launch_bounds__(256, WAVES) void rb_dq_kernel(RbArgs a) {
       if (u == 0) transfer();
       u32x4 kf[2][ND];
 #pragma unroll
-      for (int kk = 0; kk < (DP == 128 ? 0 : 2); ++kk)
+      for (int kk = 0; kk < (LATE ? 0 : 2); ++kk)
 #pragma unroll
         for (int d = 0; d < ND; ++d) kf[kk][d] = in.frag_t(kt, 32 * u + 16 * kk, d);
       __builtin_amdgcn_sched_barrier(0);
@@ -945,11 +952,12 @@ __global__ __launch_bounds__(256, WAVES) void rb_dq_kernel(RbArgs a) {
       if constexpr (E::narrow) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] *= fac;
+        fit(s, dq, fac);
       }
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         const u32x4 ds = pack8<E>(s, 8 * kk);
-        if (DP == 128) {  // (no registers to hold them across the exponentials)
+        if (LATE) {
 #pragma unroll
           for (int d = 0; d < ND; ++d) kf[kk][d] = in.frag_t(kt, 32 * u + 16 * kk, d);
         }
@@ -1066,8 +1074,7 @@ __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
   unsigned char* const sO = smem + 2 * TILE;
   unsigned char* const sV = smem + 4 * TILE;  // [128 keys] of V (WIDE)
   float* const sL = reinterpret_cast<float*>(sV + (WIDE ? 128 * P : 0));  // [2][2][64] lse2 | -delta of a tile's rows
-  float* const sF = sL + 256;                                   // [2] largest sum of squares of a tile's rows of dout (fp16)
-  float* const sB = sF + 4;
+  float* const sB = sL + 256;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, n32 = lane & 31;
   const Place at = place_of(a);
   const Quot bh = split(at.head, a.per_head);
@@ -1096,7 +1103,7 @@ __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
       dV.next(lds_addr(sV) + 64 * P, wave);
     }
   }
-  float lrow = 0.f, fac = 2e37f;  // fac (fp16): above every factor until a gradient has been seen
+  float lrow = 0.f, fac = RB_FAC0;  // fac: of the rounded dS (fp16)
 
   for (int it = it0; it < it1;) {
     const int g = it / per, ta = t0 + it % per, tb = min(t0 + per, ta + it1 - it);  // one head's run of tiles
@@ -1105,19 +1112,14 @@ __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
     TileDma<DP, ROWS> dQ, dO;
     dQ.init(a.q + b * a.sq.b + h * a.sq.h, a.sq.t, ta, sq.qlen, a.D, wave, lane);
     dO.init(a.dout + b * a.sdo.b + h * a.sdo.h, a.sdo.t, ta, sq.qlen, a.D, wave, lane);
-    constexpr int STATS = E::narrow ? 3 : 2;  // waves that bring a tile's row statistics
-    const float* const rl = (wave == 0 ? a.lse2 : wave == 1 ? a.delta : a.size) + ((int64_t)b * a.H + h) * a.tq128;
+    const float* const rl = (wave == 0 ? a.lse2 : a.delta) + ((int64_t)b * a.H + h) * a.tq128;  // two waves bring a tile's row statistics
     auto load = [&](int t, int buf) {
       dQ.next(lQ + buf * TILE, wave);
       dO.next(lO + buf * TILE, wave);
-      if (wave < STATS) lrow = rl[t * ROWS + (lane & (ROWS - 1))];
+      if (wave < 2) lrow = rl[t * ROWS + (lane & (ROWS - 1))];
     };
     auto store = [&](int buf) {
       if (wave < 2) sL[buf * 128 + wave * 64 + lane] = lrow;
-      if (E::narrow && wave == 2) {
-        const float top = wave_max(lrow);
-        if (lane == 0) sF[buf] = top;
-      }
     };
     __syncthreads();  // the head before has been read
     load(ta, 0);
@@ -1131,17 +1133,6 @@ __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
       const bool more = t + 1 < tb;
       if (more) load(t + 1, buf ^ 1);
       constexpr unsigned qt = buf * TILE, ot = (2 + buf) * TILE;
-      if constexpr (E::narrow) {  // one factor for all of dK's sum so far: a tile of larger gradients takes it down
-        const float top = sF[buf], f = row_factor(top);
-        if (top > 0.f && f < fac) {
-          const float down = fac > 1e37f ? 0.f : f / fac;
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) dk[d][r] *= down;
-          fac = f;
-        }
-      }
 #pragma unroll
       for (int u = 0; u < ROWS / 32; ++u) {
         const int p0 = sq.off + t * ROWS + 32 * u;  // position of the sub-tile's first query
@@ -1222,6 +1213,7 @@ __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
           for (int r = n * M; r < (n + 1) * M; ++r) dp[r] *= E::narrow ? s[r] * fac : s[r];
           __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (E::narrow) fit(dp, dk, fac);
         xb[0] = pack8<E>(dp, 0), xb[1] = pack8<E>(dp, 8);
 #pragma unroll
         for (int n = 0; n < 2 * ND; ++n) {
@@ -1357,7 +1349,7 @@ RbArgs to_args(const csship_relbias* p) {
 
 size_t fwd_lds(int DP, int md) { return (size_t)4 * 64 * 2 * DP + (2 * (md + RB_PAD) + 1) * 4; }
 size_t dq_lds(int DP, int md) { return (size_t)4 * 64 * 2 * DP + (size_t)(md + RB_PAD + 1) * 16 + 8192 + 96; }
-size_t dkv_lds(int DP, int md) { return fwd_lds(DP, md) + 1024 + 16; }
+size_t dkv_lds(int DP, int md) { return fwd_lds(DP, md) + 1024; }
 
 // launches with more than 64 KB of LDS have to be allowed, per device: asked for at each such launch
 template <class K>
@@ -1506,7 +1498,7 @@ size_t csship_relbias_bwd_workspace(const csship_relbias* p) {
   const int64_t sums_k = splits == 1 ? 0 : (int64_t)splits * 2 * p->B * p->Hk * p->Tk * width_of(p->D);
   const int64_t sums_q = qsplits == 1 ? 0 : (int64_t)qsplits * p->B * p->H * p->Tq * width_of(p->D);
   const int64_t sums = sums_k > sums_q ? sums_k : sums_q;  // one after the other in the same memory
-  return (size_t)(3 * row_words(p) + part_words(p) + sums) * 4 + 16;
+  return (size_t)(2 * row_words(p) + part_words(p) + sums) * 4 + 16;
 }
 
 int csship_relbias_bwd(const csship_relbias* p, const uint16_t* out, const int64_t* out_stride, const float* lse, const uint16_t* dout,
@@ -1534,8 +1526,7 @@ int csship_relbias_bwd(const csship_relbias* p, const uint16_t* out, const int64
   a.dtable = dtable;
   a.delta = static_cast<float*>(workspace);
   a.lse2 = a.delta + row_words(p);
-  a.size = a.lse2 + row_words(p);
-  a.part = a.size + row_words(p);
+  a.part = a.lse2 + row_words(p);
   a.part2 = a.part + part_words(p);
   return p->dtype == CSSHIP_RELBIAS_BF16 ? bwd_by_width<ElemBf>(a, p, as_stream(stream)) : bwd_by_width<ElemHf>(a, p, as_stream(stream));
 }

@@ -1,0 +1,87 @@
+"""Attention with a bucketed relative-position bias: values far from 1 - small and large probabilities, gradients, values, scales -
+against the definition in 64 bits.
+
+u = 2^-11 is half a step of fp16 relative to the value.  Where signs are random a 2-norm over many results is compared: dq, dk and dv
+are rounded once and are sums of products whose left operand was rounded once, each rounding independent and u / sqrt(3) on
+average at most, so u sqrt(2 / 3) in all: below BOTH = 2 u = 2^-10.  What fp16 cannot hold of a result (steps of 2^-24 below 2^-14) is
+the caller's choice of scale: half a step per element, `floor`.
+"""
+import math
+
+import pytest
+import torch
+
+from test_gpu_relbias import DEV, U, make, reference, within
+
+pytestmark = pytest.mark.gpu
+
+BOTH = 2.0 ** -10
+
+
+@pytest.fixture(scope="module")
+def lib():
+    assert torch.cuda.is_available(), "GPU tests need an MI355X"
+    from css_amd import ops, ops_bwd
+    ops.lib()
+    return ops, ops_bwd
+
+
+def gradients(lib, q, k, v, table, do, buckets, **how):
+    ops, ob = lib
+    out, lse = ops.mha_relbias(q, k, v, table, buckets, want_lse=True, **how)
+    got = dict(zip(("dq", "dk", "dv", "dtable"), ob.mha_relbias_bwd(q, k, v, table, out, lse, do, buckets, **how)))
+    return got, reference(q, k, v, table, buckets, dout=do, out=out, **how)
+
+
+def near(name, got, want):
+    # beyond 65504 fp16 has nothing but infinities: both sides are cut there, which brings no two numbers further apart
+    got, want = got.cpu().double().clamp(-65504, 65504), want.clamp(-65504, 65504)
+    floor = want.numel() ** 0.5 * 2.0 ** -25
+    off, size = float((got - want).norm()), float(want.norm())
+    assert off < BOTH * size + floor, f"{name}: {off / size:.2e} of its norm"
+
+
+@pytest.mark.parametrize("D,Tq,Tk,size,up", [(64, 40, 6001, 0.02, 8.0), (64, 200, 6001, 0.001, 64.0), (128, 70, 3001, 0.001, 64.0),
+                                             (32, 300, 3001, 2.0 ** -14, 1024.0)])
+def test_gradients_of_small_values_and_many_keys_in_fp16(lib, D, Tq, Tk, size, up):
+    """dS = P (dout . v - delta) has the size of v / Tk, whatever dout's"""
+    q, k, v, table, do = make(32, torch.float16, 1, Tq, Tk, 2, 1, D, 32)
+    k, q, v, do = (k * 8).half(), (q / 8).half(), (v * size).half(), (do * up).half()
+    got, (ref, _) = gradients(lib, q, k, v, table, do, (32, 128))
+    for name in ("dq", "dk", "dv"):
+        near(name, got[name], ref[name])
+    # float32: a probability is off by at most (D + 3) 2^-24 |s| with |s| up to 12 in log2 units (9.4e-5 of it at 128), signs random
+    assert float((got["dtable"].cpu().double() - ref["dtable"]).norm() / ref["dtable"].norm()) < 1e-4
+
+
+@pytest.mark.parametrize("Tk", [40, 333])
+def test_gradients_of_large_values_in_fp16(lib, Tk):
+    """rows of v of norm 240000 along dout: dS in units of dout's norm is beyond fp16, dq and dk are not"""
+    q, k, v, table, do = make(33, torch.float16, 1, Tk, Tk, 2, 2, 64, 32)
+    v = (torch.where(v > 0, 30000.0, -30000.0)).half()
+    do = (v.float() * 2.0 ** -30).half()
+    table[0] = math.log(Tk)  # distance 0: about half of each row's probability
+    got, (ref, _) = gradients(lib, q, k, v, table, do, (32, 128))
+    for name in ("dq", "dk"):
+        assert torch.isfinite(got[name]).all()
+        near(name, got[name], ref[name])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_gradients_that_change_size_along_a_sum_in_fp16(lib, D):
+    """values 2^12 larger (and then as small again) along the keys, gradients 2^14 larger along the queries: the factors of dq's and
+    dk's sums go down in the middle of them, by different steps in different rows"""
+    for flip in (False, True):
+        q, k, v, table, do = make(36, torch.float16, 1, 400, 700, 2, 1, D, 32)
+        v, do = v * 2.0 ** -6, do * 2.0 ** -6
+        v[:, 300:450] *= 2.0 ** 12
+        do[:, ::3] *= 2.0 ** 5
+        do[:, 200:] *= 2.0 ** 14
+        v, do = v.half(), do.half()
+        if flip:
+            v, do = v.flip(1), do.flip(1)
+        got, (ref, _) = gradients(lib, q, k, v, table, do, (32, 128))
+        for name in ("dq", "dk", "dv"):
+            near(name, got[name], ref[name])
+        small = slice(200, 400) if flip else slice(0, 200)  # these rows of dq by themselves
+        near("dq of small gradients", got["dq"][:, small], ref["dq"][:, small])
