@@ -45,8 +45,9 @@ struct ElemBf {
   DEV float lo(unsigned u) { return __uint_as_float(u << 16); }
   DEV float hi(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
 };
-// fp16 reaches from 2^-24 to 2^16 only.  P is at most 1 and what rounds to zero there is below 2^-25 of its row; dS has the size of
-// dout v / Tk, which may be anything: it is multiplied by a power of two before it is rounded, and the sums are divided by it (fit).
+// fp16 reaches from 2^-24 to 2^16 only.  In the forward P is at most 1 and what rounds to zero there is below 2^-25 of its row.  In
+// the backward dS has the size of dout v / Tk, which may be anything, and a key may have little of every row's P: both are
+// multiplied by a power of two before they are rounded, and the sums are divided by it (fit).
 struct ElemHf {
   static constexpr bool narrow = true;
   DEV f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
@@ -1103,7 +1104,7 @@ __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
       dV.next(lds_addr(sV) + 64 * P, wave);
     }
   }
-  float lrow = 0.f, fac = RB_FAC0;  // fac: of the rounded dS (fp16)
+  float lrow = 0.f, fac = RB_FAC0, facP = RB_FAC0;  // of the rounded dS and P (fp16)
 
   for (int it = it0; it < it1;) {
     const int g = it / per, ta = t0 + it % per, tb = min(t0 + per, ta + it1 - it);  // one head's run of tiles
@@ -1203,6 +1204,13 @@ __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
           for (int r = n * EACH; r < (n + 1) * EACH; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, -ls[r >> 2][r & 3]));
           __builtin_amdgcn_sched_barrier(0);
         }
+        float each = 1.f;  // from P as it is multiplied to dS's factor
+        if constexpr (E::narrow) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] *= facP;
+          fit(s, dv, facP);
+          each = fac * __uint_as_float(0x7f000000u - __float_as_uint(facP));  // (fac / facP: the reciprocal of a power of two)
+        }
         u32x4 xb[2] = {pack8<E>(s, 0), pack8<E>(s, 8)};
 #pragma unroll
         for (int n = 0; n < 2 * ND; ++n) {
@@ -1210,7 +1218,7 @@ __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
           if (N2 + n + RING < N4) ring[(N2 + n) % RING] = fetch(N2 + n + RING);
           constexpr int M = 8 / ND;
 #pragma unroll
-          for (int r = n * M; r < (n + 1) * M; ++r) dp[r] *= E::narrow ? s[r] * fac : s[r];
+          for (int r = n * M; r < (n + 1) * M; ++r) dp[r] *= E::narrow ? s[r] * each : s[r];
           __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (E::narrow) fit(dp, dk, fac);
@@ -1232,11 +1240,11 @@ __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
     }
   }
   if constexpr (E::narrow) {
-    const float f = 1.f / fac;
+    const float f = 1.f / fac, fP = 1.f / facP;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dk[d][r] *= f;
+      for (int r = 0; r < 16; ++r) dk[d][r] *= f, dv[d][r] *= fP;
   }
   table_sum(a, blockIdx.x * 4 + wave, a.B * a.nqtile);  // each wave one entry of the table's gradient, from the dq kernel's shares
   if (j >= a.Tk) return;

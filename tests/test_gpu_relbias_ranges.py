@@ -41,6 +41,20 @@ def near(name, got, want):
     assert off < BOTH * size + floor, f"{name}: {off / size:.2e} of its norm"
 
 
+@pytest.mark.parametrize("D,far,gap,up", [(64, 6001, -9.0, 1024.0), (64, 6001, -6.0, 1024.0), (120, 3001, -9.0, 1024.0),
+                                          (32, 3001, -14.0, 8192.0)])
+def test_value_gradients_of_weakly_attended_keys_in_fp16(lib, D, far, gap, up):
+    """keys beyond a distance get little of every query: some 2^-22 at -9, 2^-29 (below all that fp16 holds) at -14"""
+    B, Tq, H = 1, 300, 2
+    q, k, v, table, do = make(31, torch.float16, B, Tq, far, H, 1, D, 32)
+    do = (do * up).half()
+    table[15] = table[31] = gap  # the last bucket of either side
+    got, (ref, _) = gradients(lib, q, k, v, table, do, (32, 128))
+    behind = Tq + 128
+    near("dv far", got["dv"][:, behind:], ref["dv"][:, behind:])
+    near("dv near", got["dv"][:, :behind], ref["dv"][:, :behind])
+
+
 @pytest.mark.parametrize("D,Tq,Tk,size,up", [(64, 40, 6001, 0.02, 8.0), (64, 200, 6001, 0.001, 64.0), (128, 70, 3001, 0.001, 64.0),
                                              (32, 300, 3001, 2.0 ** -14, 1024.0)])
 def test_gradients_of_small_values_and_many_keys_in_fp16(lib, D, Tq, Tk, size, up):
