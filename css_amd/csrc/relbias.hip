@@ -38,6 +38,7 @@ using False = Const<0>;
 
 struct ElemBf {
   static constexpr bool narrow = false;  // exponents as wide as f32's
+  static constexpr float up = 0.f, grow = 8.f;  // forward, log2: P of the reference, and how far a score may outgrow it
   DEV f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -45,11 +46,13 @@ struct ElemBf {
   DEV float lo(unsigned u) { return __uint_as_float(u << 16); }
   DEV float hi(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
 };
-// fp16 reaches from 2^-24 to 2^16 only.  In the forward P is at most 1 and what rounds to zero there is below 2^-25 of its row.  In
-// the backward dS has the size of dout v / Tk, which may be anything, and a key may have little of every row's P: both are
+// fp16 reaches from 2^-24 to 2^16 only.  In the forward P is 2^7 at a row's reference and up to 2^14 (2^16 if the exponents of scores of
+// 2^24 are off by a step): what rounds to zero is below 2^-32 of the reference, rows of one large and thousands of small P keep
+// the latter.  In the backward dS has the size of dout v / Tk, which may be anything, and a key may have little of every row's P: both are
 // multiplied by a power of two before they are rounded, and the sums are divided by it (fit).
 struct ElemHf {
   static constexpr bool narrow = true;
+  static constexpr float up = 7.f, grow = 7.f;
   DEV f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -317,7 +320,7 @@ DEV void store_rows(const RbArgs& a, const f32x16 (&o)[DP / 32], float m, float 
       else store4<E>(op + c, o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv);
     }
   if (a.lse != nullptr && hi == 0)
-    a.lse[((int64_t)b * a.H + h) * a.Tq + i] = sum == 0.f ? -RB_INF : (m * a.c2 + __builtin_amdgcn_logf(sum)) * RB_LN2;
+    a.lse[((int64_t)b * a.H + h) * a.Tq + i] = sum == 0.f ? -RB_INF : (m * a.c2 - E::up + __builtin_amdgcn_logf(sum)) * RB_LN2;
 }
 
 // =============================================================================================== forward
@@ -434,8 +437,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
 #pragma unroll
         for (int u = 0; u < 2; ++u) mx[u] = fmaxf(fmaxf(mx[u], s[u][r]), s[u][r + 1]);
       const float top = half_max(fmaxf(mx[0], mx[1])) + cb;
-      // the running reference moves only when some row's scores outgrow it by 2^8: probabilities stay below 256, the sums in f32
-      if (__any((top - m) * a.c2 > 8.f)) {
+      // the running reference moves only when some row's scores outgrow it by 2^8 (2^7): probabilities stay below 256 (2^14), the
+      // sums in f32
+      if (__any((top - m) * a.c2 > E::grow)) {
         const float up = fmaxf(m, top);
         const float al = up == -RB_INF ? 1.f : __builtin_amdgcn_exp2f((m - up) * a.c2);
         m = up;
@@ -445,7 +449,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[d][r] *= al;
       }
-      const float mc = ((m == -RB_INF ? 0.f : m) - cb) * a.c2;
+      const float mc = ((m == -RB_INF ? 0.f : m) - cb) * a.c2 - E::up;
       u32x4 pb[4];
       float sum[2] = {0.f, 0.f};
 #pragma unroll
@@ -595,7 +599,7 @@ __global__ __launch_bounds__(64 * NW, 2) void rb_few_kernel(RbArgs a) {
 #pragma unroll
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
     mx = half_max(mx);
-    if (__any((mx - m) * a.c2 > 8.f)) {  // as in rb_fwd_kernel
+    if (__any((mx - m) * a.c2 > E::grow)) {  // as in rb_fwd_kernel
       const float up = fmaxf(m, mx);
       const float al = up == -RB_INF ? 1.f : __builtin_amdgcn_exp2f((m - up) * a.c2);
       m = up;
@@ -605,7 +609,7 @@ __global__ __launch_bounds__(64 * NW, 2) void rb_few_kernel(RbArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= al;
     }
-    const float mc = m == -RB_INF ? 0.f : m * a.c2;
+    const float mc = (m == -RB_INF ? 0.f : m * a.c2) - E::up;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, -mc));
@@ -665,7 +669,7 @@ __global__ __launch_bounds__(64 * NW, 2) void rb_few_kernel(RbArgs a) {
     }
     if (a.nsplit > 1) {  // O rows [row][split][DP], then (reference, sum) [row][split]
       *reinterpret_cast<f32x4*>(a.part + ((first + r) * a.nsplit + part) * DP + c) = y;
-      if (c == 0) ml[(first + r) * a.nsplit + part] = make_float2(top * a.c2, sum);
+      if (c == 0) ml[(first + r) * a.nsplit + part] = make_float2(top * a.c2 - E::up, sum);
       continue;
     }
     const int64_t hq = hk * G + rr % G, iq = rr / G;
@@ -676,7 +680,7 @@ __global__ __launch_bounds__(64 * NW, 2) void rb_few_kernel(RbArgs a) {
       else store4<E>(op, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
     }
     if (c == 0 && a.lse != nullptr)
-      a.lse[((int64_t)b * a.H + hq) * a.Tq + iq] = sum == 0.f ? -RB_INF : (top * a.c2 + __builtin_amdgcn_logf(sum)) * RB_LN2;
+      a.lse[((int64_t)b * a.H + hq) * a.Tq + iq] = sum == 0.f ? -RB_INF : (top * a.c2 - E::up + __builtin_amdgcn_logf(sum)) * RB_LN2;
   }
 }
 

@@ -99,3 +99,23 @@ def test_gradients_that_change_size_along_a_sum_in_fp16(lib, D):
             near(name, got[name], ref[name])
         small = slice(200, 400) if flip else slice(0, 200)  # these rows of dq by themselves
         near("dq of small gradients", got["dq"][:, small], ref["dq"][:, small])
+
+
+def test_one_key_with_nearly_all_of_a_row_in_fp16(lib):
+    """The first key takes each row, its value is 0; the others have 2^-25.5 of it each, and the sum of thousands of them is the
+    result.  Tolerance: fp16 holds P down to 2^-32 of the row's largest in steps of that size (n 2^-32 max|v|), else as everywhere."""
+    ops, _ = lib
+    for B, Tq, Tk, H in ((1, 1000, 1000, 16), (2, 3, 4000, 4), (1, 200, 900, 2)):
+        q = torch.ones(B, Tq, H, 64, device=DEV).half()
+        k = (torch.randn(B, Tk, H, 64, generator=torch.Generator().manual_seed(34)).to(DEV) * 0.05).half()
+        k[:, 0] = 25.5 * math.log(2.0) / 8
+        v = torch.full((B, Tk, H, 64), 1000.0, device=DEV).half()
+        v[:, 0] = 0
+        table = torch.zeros(32, H, device=DEV)
+        out, lse = ops.mha_relbias(q, k, v, table, (32, 128), want_lse=True)
+        ref, mag = reference(q, k, v, table, (32, 128))
+        want, got = ref["out"], out.cpu().double()
+        tol = 1.01 * U[torch.float16] * want + (U[torch.float16] + 4e-4) * mag["out"] + Tk * 2.0 ** -32 * 1000.0 + 1e-6
+        worst = float(((got - want).abs() / tol).max())
+        assert worst <= 1.0, (B, Tq, Tk, H, worst)
+        assert float((lse.cpu().double() - ref["lse"]).abs().max()) < 1e-4
