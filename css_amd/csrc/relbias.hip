@@ -112,13 +112,15 @@ DEV int swz(int r) {
 template <int DP>
 DEV int tile_at(int r, int c) { return r * (2 * DP) + ((c ^ swz<DP>(r)) << 4); }
 
-// the sequence's lengths and query offset; values outside the tensors' extents are cut to them
+// the sequence's lengths and query offset; values outside the tensors' extents are cut to them.  Keys behind the last query's
+// position are seen by none under `causal` and count as behind the sequence's end: a cache may hold anything there.
 struct Seq { int qlen, klen, off; };
 DEV Seq seq_of(const RbArgs& a, int b) {
   Seq s;
   s.klen = a.k_lens ? min(max(a.k_lens[b], 0), a.Tk) : a.Tk;
   s.qlen = a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq;
   s.off = min(max(a.offsets ? a.offsets[b] : a.offset, -RB_MAX_POS), RB_MAX_POS);
+  if (a.causal) s.klen = min(s.klen, max(s.off + s.qlen, 0));
   return s;
 }
 

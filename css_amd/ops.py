@@ -395,8 +395,9 @@ def mha_relbias(q, k, v, table, buckets, *, scale=None, causal=False, offset=0, 
     q [B,Tq,H,D], k / v [B,Tk,Hk,D] bf16 or fp16, Hk dividing H (grouped heads), D a multiple of 8 up to 128; strided views (a
     packed q|k|v projection, a cache) are read in place.  table f32 [n_buckets, H]; buckets = (n_buckets, max_distance[,
     two_sided=True]).  scale: D ** -0.5 unless given.  Query i sits at position i + offset, key j at j (offset: a number or int32
-    [B] on the device; streaming: frames kept so far); causal: keys behind the query's position are not seen.  k_lens / q_lens
-    int32 [B]: lengths of a padded batch; what lies behind them is not read, and those rows of the result are zeros.
+    [B] on the device; streaming: frames kept so far); causal: keys behind the query's position are not seen, and those behind the
+    last query's are not read.  k_lens / q_lens int32 [B]: lengths of a padded batch; what lies behind them is not read, and those rows
+    of the result are zeros.  Keys and values that any query of a sequence sees must be finite.
     A query without keys gets zeros (log-sum-exp -inf).  -> out [B,Tq,H,D], or (out, lse f32 [B,H,Tq]) with want_lse."""
     p, q, k, v, table = _relbias_pack(q, k, v, table, buckets, scale, causal, offset, k_lens, q_lens)
     at = q.get_device()

@@ -1155,7 +1155,8 @@ void csship_debug_stamps(void* device_buffer);
  * bucket_range[n][1] of those 2 max_distance + 1 (equal bounds: none); a bucket's distances have to be contiguous.
  * k_lens / q_lens int32 [B] or NULL (all Tk / Tq); values are cut to 0 .. Tk / Tq.  offsets int32 [B], or NULL: `offset` for
  * all; cut to +-2^28.  What lies behind a sequence's end in q, k, v, out, dout is never read into a result: it may hold
- * anything; results there are zeros (lse -inf).  A key that is only masked by `causal` must hold finite values.
+ * anything; results there are zeros (lse -inf).  With `causal` this holds for keys behind the last query's position too; a key that
+ * some of a sequence's queries see must hold finite values for all of them.
  * A table entry of -2^20 or less bans its distances (the pairs drop out, their gradient is 0); one above 2^20 counts as 2^20.
  * Every sum is in a fixed order: results do not change from run to run. */
 #define CSSHIP_RELBIAS_BF16 0

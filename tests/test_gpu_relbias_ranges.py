@@ -119,3 +119,24 @@ def test_one_key_with_nearly_all_of_a_row_in_fp16(lib):
         worst = float(((got - want).abs() / tol).max())
         assert worst <= 1.0, (B, Tq, Tk, H, worst)
         assert float((lse.cpu().double() - ref["lse"]).abs().max()) < 1e-4
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_cache_that_is_not_yet_written_behind_the_newest_frame(lib, dtype):
+    """causal, no lengths: keys behind every query's position are seen by none and may hold anything, as an allocated cache does"""
+    ops, ob = lib
+    for B, Tq, H, Hk, D, T, off in ((2, 5, 4, 2, 64, 700, 333), (1, 100, 2, 1, 64, 200, 29), (2, 1, 8, 2, 128, 3000, 0), (1, 300, 4, 4, 32, 310, -2)):
+        q, k, v, table, do = make(35, dtype, B, Tq, T, H, Hk, D, 32)
+        n = off + Tq
+        k[:, n:], v[:, n:] = math.nan, math.inf
+        each = torch.full((B,), off, dtype=torch.int32, device=DEV)
+        lens = torch.full((B,), n, dtype=torch.int32)
+        for o in (off, each):
+            out, lse = ops.mha_relbias(q, k, v, table, (32, 128), want_lse=True, causal=True, offset=o)
+            got = dict(zip(("dq", "dk", "dv", "dtable"), ob.mha_relbias_bwd(q, k, v, table, out, lse, do, (32, 128), causal=True, offset=o)))
+            ref, mag = reference(q, k, v, table, (32, 128), causal=True, offset=off, k_lens=lens, dout=do, out=out)
+            within("out", out, ref["out"], mag["out"], dtype, T, float(v[:, :n].float().abs().max()))
+            for name, top in (("dq", k[:, :n]), ("dk", q), ("dv", do)):
+                within(name, got[name], ref[name], mag[name], dtype, T * H // Hk, float(top.float().abs().max()))
+            assert torch.isfinite(got["dtable"]).all()
+            assert (got["dk"][:, n:] == 0).all() and (got["dv"][:, n:] == 0).all()
