@@ -1332,6 +1332,7 @@ int check_args(const csship_relbias* p) {
   if (p->dtype != CSSHIP_RELBIAS_BF16 && p->dtype != CSSHIP_RELBIAS_FP16) return CSSHIP_EUNSUPPORTED;
   if (p->n_buckets < 2 || p->n_buckets > 32767 || p->max_distance < 1 || p->max_distance > CSSHIP_RELBIAS_MAX_DISTANCE)
     return CSSHIP_EUNSUPPORTED;
+  if ((int64_t)p->n_buckets * p->H > 0x7fffffff) return CSSHIP_EBADSHAPE;  // the table's indexes are 32-bit
   if (!(p->scale > 1e-6f && p->scale < 1e6f)) return CSSHIP_EUNSUPPORTED;
   if (p->table == nullptr || p->bucket_of == nullptr) return CSSHIP_ENULL;
   const bool rows = p->B > 0 && p->Tq > 0, keys = p->B > 0 && p->Tk > 0;
@@ -1520,6 +1521,7 @@ int csship_relbias_bwd(const csship_relbias* p, const uint16_t* out, const int64
                        uint16_t* dv, const int64_t* dv_stride, float* dtable, void* workspace, size_t workspace_bytes,
                        csship_stream_t stream) {
   if (const int rc = check_args(p)) return rc;
+  if ((int64_t)p->n_buckets * p->H > (1 << 26) - 4) return CSSHIP_EBADSHAPE;  // a wave for each entry: fewer than 2^32 threads
   const bool rows = p->B > 0 && p->Tq > 0, keys = p->B > 0 && p->Tk > 0;
   if (p->bucket_range == nullptr || dtable == nullptr || out_stride == nullptr || dout_stride == nullptr || dq_stride == nullptr ||
       dk_stride == nullptr || dv_stride == nullptr || workspace == nullptr)

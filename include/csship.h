@@ -1150,6 +1150,7 @@ void csship_debug_stamps(void* device_buffer);
  * q, out, dout, dq [B, Tq, H, D]; k, v, dk, dv [B, Tk, Hk, D], bf16 or fp16 (dtype), strides in ELEMENTS for (sequence, frame,
  * head), the last dimension dense; strides are non-negative multiples of 8, the frame stride from D to below 2^23, inputs 16-byte and
  * results 8-byte aligned.  D is a multiple of 8 up to 128.  lse f32 [B, H, Tq] dense.  table, dtable f32 [n_buckets, H] dense.
+ * n_buckets H stays below 2^31, in the backward below 2^26 - 3.
  * bucket_of int16 [2 max_distance + 1]: the bucket of r at bucket_of[r + max_distance]; distances beyond +-max_distance take the
  * end entries.  bucket_range int32 [n_buckets][2] (backward): bucket n holds the distances bucket_range[n][0] <= r <
  * bucket_range[n][1] of those 2 max_distance + 1 (equal bounds: none); a bucket's distances have to be contiguous.

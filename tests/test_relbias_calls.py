@@ -3,7 +3,7 @@ import threading
 
 import torch
 
-from css_amd import ops
+from css_amd import _lib, ops
 
 
 def test_two_threads_at_first_use_get_the_tables_that_are_kept(monkeypatch):
@@ -31,3 +31,21 @@ def test_two_threads_at_first_use_get_the_tables_that_are_kept(monkeypatch):
     (kept,) = ops._RELBIAS_BUCKETS.values()
     for g in got:
         assert g is not None and all(a is b for a, b in zip(g, kept))
+
+
+def packed(B, Tq, Tk, H, Hk, D, n, q_stride=None, k_stride=None):
+    """csship_relbias with addresses that are never used"""
+    q_stride, k_stride = q_stride or (Tq * H * D, H * D, D), k_stride or (Tk * Hk * D, Hk * D, D)
+    return _lib.RELBIAS.pack(256, 256, 256, *q_stride, *k_stride, *k_stride, 256, 256, 256, 0, 0, 0, _lib.RELBIAS_BF16, B, Tq, Tk, H, Hk, D,
+                             n, 128, 0, 0, 1.0)
+
+
+def test_tables_beyond_32_bit_indexes_are_refused():
+    """heads x buckets number the table's entries in 32 bits in the kernels, and the backward's grid by waves"""
+    h, bad = _lib.lib(), -1
+    s3 = _lib.STRIDE3.pack(8, 8, 8)
+    for H, n, fwd, bwd in ((600000, 4094, False, False), (65536, 32767, True, False), (4096, 16384, True, False), (4096, 16383, True, True)):
+        p = packed(1, 1, 1, H, 1, 8, n, q_stride=(H * 8, H * 8, 8))
+        # a null result is refused only behind the shape: nothing is launched either way
+        assert (h.csship_relbias_fwd(p, None, s3, None, None, 0, None) == bad) == (not fwd)
+        assert (h.csship_relbias_bwd(p, *[256, s3, 256, 256, s3, 256, s3, 256, s3, 256, s3], None, 256, 0, None) == bad) == (not bwd)
