@@ -304,10 +304,14 @@ _RELBIAS_BUCKETS = {}  # (device index, n_buckets, max_distance, two_sided) -> (
 def relbias_buckets(buckets, device):
     """(bucket_of int16, bucket_range int32 [n, 2]) of csship_relbias on ``device`` for buckets = (n_buckets, max_distance[,
     two_sided]).  Built at the first call with these settings, which therefore must not be under graph capture."""
+    if not isinstance(buckets, (tuple, list)) or not 1 < len(buckets) < 4:
+        raise RuntimeError(f"css_amd: buckets {buckets}: (number of buckets, largest distance[, two-sided])")
     n, far, two = (*buckets, True)[:3]
-    key = (device.index, int(n), int(far), bool(two))
-    got = _RELBIAS_BUCKETS.get(key)
+    got = _RELBIAS_BUCKETS.get((device.index, n, far, bool(two)))
     if got is None:
+        if isinstance(n, str) or isinstance(far, str) or n != int(n) or far != int(far):
+            raise RuntimeError(f"css_amd: buckets {buckets}: whole numbers")
+        key = (device.index, int(n), int(far), bool(two))
         m = relbias_bucket_map(n, far, two)
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("css_amd: first use of these bucket settings under graph capture: call ops.relbias_buckets before it")
@@ -362,6 +366,7 @@ def _relbias_pack(q, k, v, table, buckets, scale, causal, offset, k_lens, q_lens
     if D % 8 or not 8 <= D <= 128:
         raise RuntimeError(f"css_amd: head width {D}: a multiple of 8 up to 128")
     _need(table, torch.float32, "table")
+    bucket_of, bucket_range = relbias_buckets(buckets, q.device)
     n, far = int(buckets[0]), int(buckets[1])
     if tuple(table.shape) != (n, H) or table.get_device() != q.get_device():
         raise RuntimeError(f"css_amd: 'table' must be [{n}, {H}] on {q.device}, got {tuple(table.shape)} on {table.device}")
@@ -377,7 +382,6 @@ def _relbias_pack(q, k, v, table, buckets, scale, causal, offset, k_lens, q_lens
     scale = D ** -0.5 if scale is None else float(scale)
     if not 1e-6 < scale < 1e6:
         raise RuntimeError(f"css_amd: scale {scale}: a positive number of ordinary size")
-    bucket_of, bucket_range = relbias_buckets(buckets, q.device)
     p = _lib.RELBIAS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
                           table.data_ptr(), bucket_of.data_ptr(), bucket_range.data_ptr(), kl, ql, each,
                           _lib.RELBIAS_BF16 if q.dtype is torch.bfloat16 else _lib.RELBIAS_FP16, B, Tq, Tk, H, Hk, D, n, far,

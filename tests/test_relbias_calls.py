@@ -1,6 +1,7 @@
 """Attention with a bucketed relative-position bias, host side: the bucket tables shared by threads and the argument checks."""
 import threading
 
+import pytest
 import torch
 
 from css_amd import _lib, ops
@@ -49,3 +50,11 @@ def test_tables_beyond_32_bit_indexes_are_refused():
         # a null result is refused only behind the shape: nothing is launched either way
         assert (h.csship_relbias_fwd(p, None, s3, None, None, 0, None) == bad) == (not fwd)
         assert (h.csship_relbias_bwd(p, *[256, s3, 256, 256, s3, 256, s3, 256, s3, 256, s3], None, 256, 0, None) == bad) == (not bwd)
+
+
+@pytest.mark.parametrize("buckets", [(32, 128, True, 4), (32,), (32.5, 128), (32, 128.5, True), ("32", 128), 32, None])
+def test_malformed_bucket_settings_are_refused(buckets, monkeypatch):
+    """not cut to the first three, not rounded"""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    with pytest.raises((RuntimeError, TypeError), match="buckets"):
+        ops.relbias_buckets(buckets, torch.device("cpu"))
