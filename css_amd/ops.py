@@ -302,11 +302,15 @@ _RELBIAS_BUCKETS = {}  # (device index, n_buckets, max_distance, two_sided) -> (
 
 
 def relbias_buckets(buckets, device):
-    """(bucket_of int16, bucket_range int32 [n, 2]) of csship_relbias on ``device`` for buckets = (n_buckets, max_distance[,
+    """(bucket_of int16, bucket_range int32 [n, 2]) of csship_relbias on ``device`` ("cuda": the current one) for buckets = (n_buckets, max_distance[,
     two_sided]).  Built at the first call with these settings, which therefore must not be under graph capture."""
     if not isinstance(buckets, (tuple, list)) or not 1 < len(buckets) < 4:
         raise RuntimeError(f"css_amd: buckets {buckets}: (number of buckets, largest distance[, two-sided])")
     n, far, two = (*buckets, True)[:3]
+    if not isinstance(device, torch.device) or device.index is None:
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:  # the tensors' devices have an index
+            device = torch.device("cuda", torch.cuda.current_device())
     got = _RELBIAS_BUCKETS.get((device.index, n, far, bool(two)))
     if got is None:
         if isinstance(n, str) or isinstance(far, str) or n != int(n) or far != int(far):

@@ -58,3 +58,16 @@ def test_malformed_bucket_settings_are_refused(buckets, monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     with pytest.raises((RuntimeError, TypeError), match="buckets"):
         ops.relbias_buckets(buckets, torch.device("cpu"))
+
+
+def test_tables_made_ahead_serve_the_device_that_is_meant(monkeypatch):
+    """a capture is prepared by ops.relbias_buckets(settings, "cuda"): the entry a tensor's device finds is that one"""
+    monkeypatch.setattr(ops, "_RELBIAS_BUCKETS", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch, "tensor", lambda x, dtype, make=torch.tensor: type("T", (), {"to": lambda self, d: make(x, dtype=dtype)})())
+    kept = ops.relbias_buckets((32, 128), torch.device("cuda", 0))
+    assert len(ops._RELBIAS_BUCKETS) == 1
+    for device in ("cuda", "cuda:0", torch.device("cuda"), 0):
+        assert ops.relbias_buckets((32, 128), device) is kept
+    assert len(ops._RELBIAS_BUCKETS) == 1
