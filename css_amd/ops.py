@@ -302,8 +302,9 @@ _RELBIAS_BUCKETS = {}  # (device index, n_buckets, max_distance, two_sided) -> (
 
 
 def relbias_buckets(buckets, device):
-    """(bucket_of int16, bucket_range int32 [n, 2]) of csship_relbias on ``device`` ("cuda": the current one) for buckets = (n_buckets, max_distance[,
-    two_sided]).  Built at the first call with these settings, which therefore must not be under graph capture."""
+    """(bucket_of int16, bucket_range int32 [n, 2]) of csship_relbias on ``device`` ("cuda": the current one) for buckets =
+    (n_buckets, max_distance[, two_sided]).  Built at the first call with these settings, which therefore must not be under graph
+    capture."""
     if not isinstance(buckets, (tuple, list)) or not 1 < len(buckets) < 4:
         raise RuntimeError(f"css_amd: buckets {buckets}: (number of buckets, largest distance[, two-sided])")
     n, far, two = (*buckets, True)[:3]

@@ -8,6 +8,7 @@ ranks -- a single large all-reduce is what the point-to-point xGMI links want (2
 ranks with no collective on the data path.
 """
 import os
+import warnings
 
 import torch
 import torch.distributed as dist
@@ -275,6 +276,17 @@ def allreduce_plan(flat, plan, average=True, async_handles=None):
         wait_all(handles, flat, average)
 
 
+def interprocess_events(n, stream):
+    """(n recorded interprocess events, None), or (None, the reason) where the runtime refuses them"""
+    try:
+        events = [torch.cuda.Event(enable_timing=False, interprocess=True) for _ in range(n)]
+        for e in events:
+            e.record(stream)
+        return events, None
+    except RuntimeError as err:
+        return None, str(err).split("\n")[0]
+
+
 class P2PAllReduce:
     """Direct (one-shot) all-reduce of FusedAdam's flat gradient buffer over peer-mapped memory - the hand-written variant
     SURVEY 5.8 keeps beside RCCL's collective (replaces scripts/python/combine_models.py:55-82).  OFF by default:
@@ -293,6 +305,10 @@ class P2PAllReduce:
         peer's event.  (1) "ready": gradients are final -> csship_p2p_reduce sums this rank's slice over all buffers
         in rank order, in place; (2) "reduced": -> the other slices are copied from their owners; (3) "done": nobody
         still reads this rank's buffer -> the call returns, the stream may overwrite the gradients.
+    A runtime that cannot record interprocess events (hipErrorInvalidValue where it may not register host memory) leaves the
+    handshake to the hosts: in each phase a rank waits for its own stream before it publishes its number, and no stream waits for
+    another process.  All ranks use one form; ``self.by_events`` says which, a warning says why.  Same results; the host, and with it
+    what the backward pass would issue meanwhile, stands still.
     Sums run in rank order 0 .. W-1 on ONE rank per slice, so every rank ends up with the same bits, whatever the timing.
     Visibility across devices rests on the event semantics of the runtime (a recorded interprocess event releases to
     system scope, a stream that waited for one acquires): nothing here reads another device's memory except behind such
@@ -313,15 +329,18 @@ class P2PAllReduce:
         self.timeout_s, self.seq = float(timeout_s), 0
         dev = flat.device
         # interprocess events: created by a first record, then exported
-        self.events = [torch.cuda.Event(enable_timing=False, interprocess=True) for _ in range(self.PHASES)]
-        for e in self.events:
-            e.record(torch.cuda.current_stream(dev))
+        self.events, refused = interprocess_events(self.PHASES, torch.cuda.current_stream(dev))
         torch.cuda.synchronize(dev)
-        mine = {"tensor": reduce_tensor(flat), "events": [e.ipc_handle() for e in self.events], "n": flat.numel()}
+        mine = {"tensor": reduce_tensor(flat), "events": self.events and [e.ipc_handle() for e in self.events], "n": flat.numel(),
+                "refused": refused}
         everyone = [None] * self.world
         dist.all_gather_object(everyone, mine)
         if any(o["n"] != flat.numel() for o in everyone):
             raise ValueError("P2PAllReduce: ranks hold gradient buffers of different sizes")
+        refused = [f"rank {j}: {o['refused']}" for j, o in enumerate(everyone) if o["refused"] is not None]
+        self.by_events = not refused
+        if refused and self.rank == 0:
+            warnings.warn("css_amd.P2PAllReduce: no interprocess events (" + "; ".join(refused) + "): the hosts wait for the streams instead")
         self.peers, self.peer_events = [], []
         for j, o in enumerate(everyone):
             if j == self.rank:
@@ -330,7 +349,7 @@ class P2PAllReduce:
             else:
                 fn, args = o["tensor"]
                 self.peers.append(fn(*args))          # this process's mapping of rank j's buffer
-                self.peer_events.append([torch.cuda.Event.from_ipc_handle(dev, h) for h in o["events"]])
+                self.peer_events.append([torch.cuda.Event.from_ipc_handle(dev, h) for h in o["events"]] if self.by_events else None)
         import ctypes as C
         self._ptrs = (C.c_void_p * self.world)(*[t.data_ptr() for t in self.peers])
         # sequence numbers [phase][rank] in shared memory (rank 0 names the file)
@@ -349,9 +368,13 @@ class P2PAllReduce:
             os.unlink(self._shm_name)   # every rank has it mapped: the name can go
 
     def _phase(self, k, stream):
-        """record my event of phase k, publish, and make `stream` wait for every peer's event of this call"""
+        """record my event of phase k, publish, and make `stream` wait for every peer's event of this call (without events: wait for
+        `stream`, publish, wait for every peer's number)"""
         import time
-        self.events[k].record(stream)
+        if self.by_events:
+            self.events[k].record(stream)
+        else:
+            stream.synchronize()
         self._seqs[k, self.rank] = self.seq
         deadline = time.monotonic() + self.timeout_s
         for j in range(self.world):
@@ -361,7 +384,8 @@ class P2PAllReduce:
                 if time.monotonic() > deadline:
                     raise RuntimeError(f"css_amd.P2PAllReduce: rank {j} did not reach phase {k} of call {self.seq} within "
                                        f"{self.timeout_s:.0f} s (ranks must issue the same all-reduces in the same order)")
-            stream.wait_event(self.peer_events[j][k])
+            if self.by_events:
+                stream.wait_event(self.peer_events[j][k])
 
     def allreduce_async(self, lo=0, hi=None, average=True):
         """The same on this reducer's own stream, ordered behind what the current stream has been given so far (the
