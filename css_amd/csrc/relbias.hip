@@ -329,10 +329,12 @@ DEV void store_rows(const RbArgs& a, const f32x16 (&o)[DP / 32], float m, float 
 // One workgroup = 4 waves x 32 queries of one (sequence, head); 64-key tiles of K and V, double buffered in LDS, softmax in one pass
 // with a running maximum and sum in f32.  P is rounded to the tensors' type as the second product's operand (half a step of each
 // term, while the sum that divides it is not rounded): f32 operands would take eight times the matrix unit's time.
-// Bound by the vector unit at 64 columns: a score takes an exponential (8 cycles a wave) and some four instructions beside its
-// 128 flops, and the two units run side by side only across waves.  11250 x 11250, 8 heads of 64: 317 us, 818 TFLOP/s (a large
-// matrix product reaches 1178 here); 2 x 2047 causal, 16 heads of 128: 55 us, 625 TFLOP/s; 32 x 400, 4 heads: 15.4 us, of which some
-// 3.4 pass before the first product.  Scores of the next tile issued ahead of this one's exponentials took 496 us for the long
+// At 64 columns the vector unit works for 62% of the busy cycles (an exponential and some four instructions a score) and the matrix
+// unit for 39%: 101% together, so on a SIMD they take turns - two or three waves do not bring them side by side.
+// 11250 x 11250, 8 heads of 64: 317 to 325 us from card to card, 800 to 818 TFLOP/s (a large matrix product reaches 1178 here).  At
+// 128 columns, 2 x 2047 causal, 16 heads: 55.6 us, 618 TFLOP/s, each unit at work for 28%: on average 1.3 waves a SIMD (two fit the
+// registers, and the row tiles end one by one), which wait for 37% of their time.  32 x 400, 4 heads: 15.2 us, of which some 3.4 pass
+// before the first product.  Scores of the next tile issued ahead of this one's exponentials took 496 us for the long
 // case: the registers of both tiles do not fit beside two waves.
 template <class E, int DP>
 __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a) {
@@ -497,8 +499,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void rb_fwd_kernel(RbArgs a
 // Nothing is reused across waves, so each of the NW waves streams its own 32-key tiles (every NW-th of the workgroup's), K straight
 // into operand registers, V through a wave's own LDS tile for the transposing reads, the next tile's loads in flight; the waves'
 // running softmax states are joined in LDS.  Bound by the bytes of K and V: 32 x 1 against up to 8192 keys, 16 heads in groups of 4,
-// 128 columns: 95.7 us, 4.16 TB/s (a large copy reaches 5.16); 4 x 8 x 30001, 8 heads of 64: 53.5 us, 4.6 TB/s; 1 x 500, 4 heads:
-// 11.7 us, one workgroup's chain of loads.  Where few workgroups would run, the keys are split over `nsplit` of them: states go
+// 128 columns: 95.5 us, 4.17 TB/s (a large copy reaches 5.16); 4 x 8 x 30001, 8 heads of 64: 53.7 us, 4.6 TB/s; 1 x 500, 4 heads:
+// 12.1 us, one workgroup's chain of loads (8.6 us).  Where few workgroups would run, the keys are split over `nsplit` of them: states go
 // to the workspace and rb_join_kernel joins them in order (4.8 us for the first of these).
 constexpr int RB_FEW_TABLE = 4096;  // floats of LDS for the group's tables by distance; wider ones are gathered from memory
 template <int DP, int NW>
@@ -760,9 +762,10 @@ DEV float swap_halves(float x) {
 // dS is rounded to the tensors' type for the last product only; the table's gradient takes it in f32.  dk and dv have a kernel of
 // their own, which computes S and dP again (7 products for 5): sums over queries and over keys in one kernel would need atomics,
 // and results that change from run to run, or a T x T operand in memory.
-// Bound by both units in turn: 6001 x 6001, 8 heads of 64: 139 us, 800 TFLOP/s of its three products, the vector unit busy for 59%
-// of the time, the matrix unit for 42%.  2 x 2047 causal, 16 heads of 128: 85 us (125 with the operands' addresses held in
-// registers, which did not fit); 32 x 400, 4 heads: 27 us.
+// Bound by both units in turn: 6001 x 6001, 8 heads of 64: 141 us, 782 TFLOP/s of its three products, the vector unit busy for 58%
+// of the time, the matrix unit for 40%.  2 x 2047 causal, 16 heads of 128: 89 us, each unit 28% (with the operands' addresses held
+// in registers, which did not fit, half as long again); 32 x 400, 4 heads: 28 to 30 us.  fp16: the factor of dS (fit) and what it
+// pushes out of the registers take 159 us instead of 151 for the first of these, 97 instead of 93 for the second.
 // Where few workgroups would run, the keys are split over `nsplit` of them, whose sums rb_dq_join_kernel adds in order.
 // It also leaves delta_i = do_i . o_i and the rows' log-sum-exp in log2 units for the next kernel, +inf where a row has no
 // keys or lies behind its sequence (exp2(s - inf) = 0: such rows drop out of every product).
@@ -823,7 +826,8 @@ __global__ __launch_bounds__(256, WAVES) void rb_dq_kernel(RbArgs a) {
     delta = half_sum(delta);
     if (x != -RB_INF) lse2 = x * RB_LOG2E;
     // The matrix unit's sums lean to the negative side by about 2^-25 each; over the 36 million pairs of a 6001 x 6001 head that
-    // showed as 10^-5 of the table's gradient.  Odd waves therefore compute -dP (and all behind it), so that it cancels.
+    // showed as 10^-5 of the table's gradient.  Odd waves therefore compute -dP (and all behind it), so that it cancels (5 10^-7 left
+    // against these formulas in 64 bits; that delta takes the rounded out costs far more, see include/csship.h).
     if (wave & 1) {
 #pragma unroll
       for (int ks = 0; ks < NK; ++ks) df[ks] ^= 0x80008000u;
@@ -1063,10 +1067,11 @@ DEV void table_sum(const RbArgs& a, int entry, int nwg) {
 // dk and dv: 4 waves x 32 keys of one (sequence, key head) against 64-query tiles of every head of its group.
 //   S = Q K^T (+ bias), dV^T += dO^T P, dP = dO V^T (from -delta), dK^T += Q^T dS
 // P and dS are rounded to the tensors' type as operands, the sums are f32.  Operands are requested ahead of their products through
-// a whole sub-tile, which else waited for LDS twelve times (6001 x 6001, 8 heads of 64: 214 -> 203 us, 725 TFLOP/s of its four products).
+// a whole sub-tile, which else waited for LDS twelve times (6001 x 6001, 8 heads of 64: 214 -> 202 us, 730 TFLOP/s of its four products).
 // WIDE: K and the sums are 160 of 256 registers, V stays in LDS and tiles have 32 rows (2 x 2047 causal, 4 key heads of 128: 91 us,
-// 750 TFLOP/s; with V in registers one wave a SIMD remains: 107).  32 x 400, 4 heads: 27 us.  Both units are busy for 35% of the
-// 6001 x 6001 case: its 376 workgroups leave every second SIMD with one wave, and 220 registers allow no third.  Where few workgroups would run, the (head, query tile) steps are split over `nsplit`
+// 750 TFLOP/s; with V in registers one wave a SIMD remains: 107).  32 x 400, 4 heads: 26 us.  Both units are busy for 35% of the
+// 6001 x 6001 case: its 376 workgroups leave every second SIMD with one wave, and 220 registers allow no third.  fp16: the factors of
+// P and dS (fit) take 242 us instead of 228 there, 110 instead of 108 at 128 columns.  Where few workgroups would run, the (head, query tile) steps are split over `nsplit`
 // workgroups, whose sums rb_dkv_join_kernel adds in order.
 template <class E, int DP>
 __global__ __launch_bounds__(256, 2) void rb_dkv_kernel(RbArgs a) {
