@@ -140,3 +140,63 @@ def test_a_cache_that_is_not_yet_written_behind_the_newest_frame(lib, dtype):
                 within(name, got[name], ref[name], mag[name], dtype, T * H // Hk, float(top.float().abs().max()))
             assert torch.isfinite(got["dtable"]).all()
             assert (got["dk"][:, n:] == 0).all() and (got["dv"][:, n:] == 0).all()
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_overflowed_and_absent_gradients(lib, dtype, D):
+    """an infinity in dout (a loss scale that was too large) is seen in every gradient it belongs to and in no other sequence's or
+    head's; a gradient of zeros gives zeros"""
+    ops, ob = lib
+    q, k, v, table, do = make(37, dtype, 2, 150, 170, 4, 2, D, 32)
+    out, lse = ops.mha_relbias(q, k, v, table, (32, 128), want_lse=True)
+    bad = do.clone()
+    bad[0, 77, 1] = math.inf
+    dq, dk, dv, dt = ob.mha_relbias_bwd(q, k, v, table, out, lse, bad, (32, 128))
+    want = ob.mha_relbias_bwd(q, k, v, table, out, lse, do, (32, 128))
+    assert not torch.isfinite(dq[0, 77, 1]).any() and not torch.isfinite(dv[0, :, 0]).any() and not torch.isfinite(dk[0, :, 0]).any()
+    assert not torch.isfinite(dt[:, 1]).all()
+    others = torch.ones(2, 150, 4, dtype=torch.bool, device=DEV)
+    others[0, 77, 1] = False
+    assert torch.equal(dq[others], want[0][others])
+    for a, b in ((dk, want[1]), (dv, want[2])):
+        assert torch.equal(a[1], b[1]) and torch.equal(a[0, :, 1], b[0, :, 1])
+    assert torch.equal(dt[:, [0, 2, 3]], want[3][:, [0, 2, 3]])
+    for g in ob.mha_relbias_bwd(q, k, v, table, out, lse, torch.zeros_like(do), (32, 128)):
+        assert (g == 0).all()
+
+
+def test_two_threads_on_streams_of_their_own(lib):
+    """forward and backward of both types at once, with settings that neither thread has used before: the same bits as alone"""
+    import threading
+    ops, ob = lib
+    jobs = []
+    for n, dtype in enumerate((torch.bfloat16, torch.float16)):
+        x = make(50 + n, dtype, 2, 200, 300, 4, 2, 64, 24)
+        jobs.append((x, torch.cuda.Stream(), []))
+    torch.cuda.synchronize()
+    together = threading.Barrier(2, timeout=30)
+
+    def work(x):
+        out, lse = ops.mha_relbias(*x[:4], (24, 119), want_lse=True)
+        step = ops.mha_relbias(x[0][:, -1:], *x[1:4], (24, 119), offset=299)
+        return (out, lse, step, *ob.mha_relbias_bwd(*x[:4], out, lse, x[4], (24, 119)))
+
+    def thread(x, stream, got):
+        with torch.cuda.stream(stream):
+            together.wait()
+            for _ in range(20):
+                got.append(work(x))
+        stream.synchronize()
+
+    threads = [threading.Thread(target=thread, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    for x, _, got in jobs:
+        alone = work(x)
+        torch.cuda.synchronize()
+        assert len(got) == 20
+        for g in got:
+            assert all(torch.equal(a, b) for a, b in zip(alone, g))
